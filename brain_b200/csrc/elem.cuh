@@ -1,0 +1,62 @@
+// Element types of the kernels that take bf16, f16 or f32 alike: conversions, 16-byte vectors, block sums.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+// dtype codes of the C entry points (brain_b200/ops/_common.py::dtype_code)
+enum BrainDtype : int { BRAIN_BF16 = 0, BRAIN_F16 = 1, BRAIN_F32 = 2 };
+
+namespace brain {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// 16 bytes of T, kept packed until used.
+template <typename T>
+struct alignas(16) Vec16 {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+
+// Sum over a block of up to 32 warps; every thread gets it. `red` holds 32 values and may be reused at once.
+template <typename A>
+__device__ __forceinline__ A block_sum_all(A v, A* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int w = threadIdx.x / 32, l = threadIdx.x % 32, nw = (blockDim.x + 31) / 32;
+  __syncthreads();
+  if (l == 0) red[w] = v;
+  __syncthreads();
+  A t = l < nw ? red[l] : A(0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
+}
+
+__device__ __forceinline__ float block_max_all(float v, float* red) {
+  v = warp_max(v);
+  const int w = threadIdx.x / 32, l = threadIdx.x % 32, nw = (blockDim.x + 31) / 32;
+  __syncthreads();
+  if (l == 0) red[w] = v;
+  __syncthreads();
+  return warp_max(l < nw ? red[l] : -INFINITY);
+}
+
+}  // namespace brain

@@ -301,6 +301,20 @@ class DistillationLoss(Loss):
         return self.alpha * kd + (1 - self.alpha) * F.cross_entropy(student.float(), labels)
 
 
+class TopKDistillationLoss(Loss):
+    """:class:`DistillationLoss` against a teacher's stored top logits (``ops.topk_distillation``): alpha * T^2
+    KL(teacher's kept entries || student_T) over the tokens that have any + (1 - alpha) * CE(student, labels)."""
+
+    def __init__(self, temperature=2.0, alpha=0.5):
+        self.T, self.alpha = temperature, alpha
+
+    def forward(self, student, teacher_logits, teacher_ids, labels=None):
+        kd = ops.topk_distillation(student, teacher_logits, teacher_ids, self.T)
+        if labels is None:
+            return kd
+        return self.alpha * kd + (1 - self.alpha) * ops.cross_entropy(student, labels)
+
+
 class MaskedLoss(Loss):
     """Apply any elementwise loss only where mask is set (masked.rs)."""
 
@@ -328,7 +342,8 @@ LOSSES = {c.__name__: c for c in [CrossEntropyLoss, NLLLoss, BCELoss, BCEWithLog
                                  KLDivLoss, CTCLoss, MSELoss, L1Loss, HuberLoss, SmoothL1Loss, LogCoshLoss,
                                  QuantileLoss, PoissonNLLLoss, GaussianNLLLoss, CosineEmbeddingLoss,
                                  MarginRankingLoss, TripletLoss, ContrastiveLoss, InfoNCELoss, NTXentLoss, DiceLoss,
-                                 CEDiceLoss, IoULoss, WassersteinLoss, GANLoss, HingeGANLoss, DistillationLoss]}
+                                 CEDiceLoss, IoULoss, WassersteinLoss, GANLoss, HingeGANLoss, DistillationLoss,
+                                 TopKDistillationLoss]}
 
 
 # ------------------------------------------------------------------ metric learning / robust / adversarial extras

@@ -48,10 +48,17 @@ _native.register({
     "brain_status_ce": ("brain_kernels", "pi"),
     "brain_status_optim": ("brain_kernels", "pi"),
     "brain_status_attention": ("brain_kernels", "pi"),
+    "brain_norm_fp8": ("brain_kernels", "iplplppppliifs"),
+    "brain_distill_rows": ("brain_kernels", "iplppppplppiliifs"),
+    "brain_distill_count": ("brain_kernels", "ppliips"),
+    "brain_distill_reduce": ("brain_kernels", "plppps"),
+    "brain_status_distill": ("brain_kernels", "pi"),
+    "brain_verify_draft": ("brain_kernels", "ipllpllpppppliis"),
+    "brain_int4_linear": ("brain_kernels", "iplplppppiiiis"),
 })
 
 STATUS_TAGS = ["gemm", "norms", "elementwise", "ce", "optim", "attention", "attention_tc", "attention_bwd_tc",
-               "attention_decode", "decode_tp"]
+               "attention_decode", "decode_tp", "distill"]
 
 
 def same_device(ref: torch.Tensor, *others) -> None:
@@ -60,6 +67,33 @@ def same_device(ref: torch.Tensor, *others) -> None:
     for t in others:
         if t is not None and t.device != ref.device:
             raise ValueError(f"tensor on {t.device} passed to a kernel running on {ref.device}")
+
+
+# codes of csrc/elem.cuh::BrainDtype
+DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def dtype_code(name: str, t: torch.Tensor, allowed=(torch.bfloat16, torch.float16, torch.float32)) -> int:
+    """The C code of ``t``'s type; TypeError naming the op for a type that its kernels do not take."""
+    if t.dtype not in allowed:
+        raise TypeError(f"{name} takes {', '.join(str(d)[6:] for d in allowed)} tensors, not {str(t.dtype)[6:]}")
+    return DTYPE_CODES[t.dtype]
+
+
+def launch(t: torch.Tensor, name: str, *args) -> None:
+    """``_native.call`` with ``t``'s device current (a launch goes to the current device) and that device's
+    current stream as the last argument."""
+    if t.device.index == torch.cuda.current_device():
+        _native.call(name, *args, _native.stream_ptr(t.device))
+    else:
+        with torch.cuda.device(t.device):
+            _native.call(name, *args, _native.stream_ptr(t.device))
+
+
+def no_backward(name: str, *tensors) -> None:
+    """Raise when autograd would record an inference op: its result would carry no gradient, silently."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def stream(t: torch.Tensor) -> int:

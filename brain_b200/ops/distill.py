@@ -1,0 +1,231 @@
+"""Distillation from a teacher's stored top logits (``csrc/distill.cu``).
+
+A teacher that was run once keeps, for each token, its k largest logits and their ids. With temperature T,
+p = softmax(teacher_logits / T) over the kept entries and q = softmax(logits / T) over the whole vocabulary,
+
+    loss = T^2 * sum_i p_i (log p_i - log q_{id_i}),    dloss/dlogits = T (q - p at its ids).
+
+``topk_distillation`` is the loss with autograd: its backward pass reads the logits again.
+``topk_distillation_grad`` gives loss and gradient of one pass over the logits, for a loop that drives the
+backward pass itself (``logits.backward(grad)``), in place if asked to. ``linear_topk_distillation`` is the LM
+head: like ``linear_cross_entropy`` it turns its one [tokens, vocab] buffer of logits into their gradient.
+
+An id of -1 is no entry (teachers that keep fewer than k), nor is a logit of -inf; a token without entries has
+loss and gradient 0 and does not count in the mean. On CUDA an id at or above the vocabulary's size is taken as
+no entry and recorded in the status words (``ops.check_status``); on the CPU it raises.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ._common import dtype_code, has_main_grad, launch, main_grad_beta, ptr, rows2d, same_device
+from .gemm import gemm
+
+MAX_TOP = 1024
+
+
+def _check(name, logits, teacher_logits, teacher_ids, temperature, reduction):
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"unknown reduction {reduction!r}")
+    if not temperature > 0 or temperature == float("inf"):
+        raise ValueError(f"{name}: temperature {temperature} is not above zero and finite")
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f"{name}: logits {tuple(logits.shape)} have no vocabulary dimension")
+    if teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != logits.shape[:-1] \
+            or teacher_ids.dim() != logits.dim():
+        raise ValueError(f"{name}: logits {tuple(logits.shape)}, teacher_logits {tuple(teacher_logits.shape)}, "
+                         f"teacher_ids {tuple(teacher_ids.shape)}")
+    if not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
+        raise ValueError(f"{name}: {teacher_ids.shape[-1]} teacher entries a token, 1 to {MAX_TOP} are taken")
+    if teacher_ids.is_floating_point() or teacher_ids.is_complex() or teacher_ids.dtype == torch.bool:
+        raise TypeError(f"{name}: teacher_ids are whole numbers")
+    if not teacher_logits.is_floating_point():
+        raise TypeError(f"{name}: teacher_logits are floating-point numbers")
+    if torch.is_grad_enabled() and teacher_logits.requires_grad:
+        raise RuntimeError(f"{name} gives the teacher no gradient: detach teacher_logits")
+    same_device(logits, teacher_logits, teacher_ids)
+
+
+def _teacher(teacher_logits, teacher_ids):
+    k = teacher_ids.shape[-1]
+    return (teacher_logits.detach().reshape(-1, k).float().contiguous(),
+            teacher_ids.reshape(-1, k).long().contiguous())
+
+
+def _rows(l2, t, ids, temperature, loss, lse, dz, grad=None, inv_n=None, grad_rows=False):
+    launch(l2, "brain_distill_rows", dtype_code("topk_distillation", l2), l2.data_ptr(), l2.stride(0), t.data_ptr(),
+           ids.data_ptr(), ptr(loss), ptr(lse), ptr(dz), 0 if dz is None else dz.stride(0), ptr(grad), ptr(inv_n),
+           int(grad_rows), l2.shape[0], t.shape[1], l2.shape[1], float(temperature))
+
+
+def _count(t, ids, V):
+    count = torch.empty(1, device=t.device, dtype=torch.int32)
+    launch(t, "brain_distill_count", t.data_ptr(), ids.data_ptr(), t.shape[0], t.shape[1], V, count.data_ptr())
+    return count
+
+
+def _reduce(loss, count, total, inv_n):
+    launch(count if loss is None else loss, "brain_distill_reduce", ptr(loss), 0 if loss is None else loss.numel(),
+           ptr(count), ptr(total), ptr(inv_n))
+
+
+def _scalar(t):
+    return torch.empty((), device=t.device, dtype=torch.float32)
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, t, ids, temperature, reduction):
+        l2 = rows2d(logits)
+        M, V = l2.shape
+        loss = torch.empty(M, device=logits.device, dtype=torch.float32)
+        lse = torch.empty_like(loss) if ctx.needs_input_grad[0] else None
+        _rows(l2, t, ids, temperature, loss, lse, None)
+        mean = reduction == "mean"
+        inv_n = _scalar(t) if mean and lse is not None else None
+        total = None
+        if reduction != "none":
+            total = _scalar(t)
+            _reduce(loss, _count(t, ids, V) if mean else None, total, inv_n)
+        ctx.save_for_backward(logits, t, ids, lse, inv_n)
+        ctx.meta = temperature, reduction
+        return loss.view(logits.shape[:-1]) if total is None else total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, t, ids, lse, inv_n = ctx.saved_tensors
+        temperature, reduction = ctx.meta
+        l2 = rows2d(logits)
+        out = torch.empty(l2.shape, device=logits.device, dtype=logits.dtype)
+        _rows(l2, t, ids, temperature, None, lse, out, g.reshape(-1).float().contiguous(), inv_n,
+              grad_rows=reduction == "none")
+        return out.view(logits.shape), None, None, None, None
+
+
+def topk_distillation_ref(logits, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
+    """Torch operations in float32 (float64 for float64 logits), differentiable."""
+    ct = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    V = logits.shape[-1]
+    if teacher_ids.numel() and int(teacher_ids.max()) >= V:
+        raise ValueError(f"teacher id {int(teacher_ids.max())} outside the vocabulary of {V}")
+    t = teacher_logits.detach().to(ct) / temperature
+    on = (teacher_ids >= 0) & (t != float("-inf"))
+    some = on.any(-1)
+    t = torch.where(on, t, torch.full_like(t, float("-inf")))
+    t = torch.where(some[..., None], t, torch.zeros_like(t))
+    logp = torch.log_softmax(t, -1)
+    p = torch.where(on, logp.exp(), torch.zeros_like(logp))
+    logq = torch.log_softmax(logits.to(ct) / temperature, -1).gather(-1, teacher_ids.long().clamp_min(0))
+    used = on & (p != 0)
+    loss = torch.where(used, p * (torch.where(used, logp, 0.0) - torch.where(used, logq, 0.0)), 0.0).sum(-1)
+    loss = loss * temperature ** 2
+    if reduction == "none":
+        return loss
+    return loss.sum() / some.sum().clamp_min(1) if reduction == "mean" else loss.sum()
+
+
+def topk_distillation(logits, teacher_logits, teacher_ids, temperature: float = 1.0, reduction: str = "mean"):
+    """Distillation loss of ``logits`` [..., V] against a teacher's kept ``teacher_logits`` [..., k] at
+    ``teacher_ids`` [..., k] (any order, at most 1024 of them); float32. ``"mean"`` is over the tokens that have
+    an entry, ``"none"`` gives the loss of each. To capture its backward pass into a CUDA graph, let go of every
+    eager loss of the same leaf first: autograd ties a leaf to the stream of its oldest living graph."""
+    _check("topk_distillation", logits, teacher_logits, teacher_ids, temperature, reduction)
+    if not logits.is_cuda:
+        return topk_distillation_ref(logits, teacher_logits, teacher_ids, temperature, reduction)
+    dtype_code("topk_distillation", logits)
+    t, ids = _teacher(teacher_logits, teacher_ids)
+    return _DistillFn.apply(logits, t, ids, float(temperature), reduction)
+
+
+def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: float = 1.0, reduction: str = "mean",
+                           out: torch.Tensor | None = None):
+    """(loss, dloss/dlogits) of :func:`topk_distillation` (with ``"none"`` the gradient of the losses' sum),
+    outside autograd. ``out`` takes the gradient: of logits' shape and type with adjacent columns, or logits
+    itself."""
+    name = "topk_distillation_grad"
+    _check(name, logits, teacher_logits, teacher_ids, temperature, reduction)
+    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.stride(-1) != 1):
+        raise ValueError(f"{name}: out {tuple(out.shape)} {out.dtype} for logits {tuple(logits.shape)} {logits.dtype}")
+    same_device(logits, out)
+    if not logits.is_cuda:
+        with torch.enable_grad():
+            z = logits.detach().requires_grad_()
+            loss = topk_distillation_ref(z, teacher_logits, teacher_ids, temperature, reduction)
+            grad = torch.autograd.grad(loss.sum(), z)[0]
+        return loss.detach(), grad if out is None else out.copy_(grad)
+    dtype_code(name, logits)
+    with torch.no_grad():
+        t, ids = _teacher(teacher_logits, teacher_ids)
+        l2 = rows2d(logits)
+        if out is None:
+            out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        o2 = out.view(-1, out.shape[-1])
+        loss, total = _loss_and_grad(l2, t, ids, temperature, reduction, o2)
+        return loss.view(logits.shape[:-1]) if total is None else total, out
+
+
+def _loss_and_grad(l2, t, ids, temperature, reduction, out):
+    loss = torch.empty(l2.shape[0], device=l2.device, dtype=torch.float32)
+    count = inv_n = total = None
+    if reduction == "mean":
+        count, inv_n = _count(t, ids, l2.shape[1]), _scalar(t)
+        _reduce(None, count, None, inv_n)
+    _rows(l2, t, ids, temperature, loss, None, out, None, inv_n)
+    if reduction != "none":
+        total = _scalar(t)
+        _reduce(loss, count, total, None)
+    return loss, total
+
+
+class _LinearDistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, w, t, ids, temperature, chunk):
+        h2 = rows2d(h)
+        M, V = h2.shape[0], w.shape[0]
+        chunk = min(chunk, M) if chunk else M
+        dlogits = torch.empty(M, -(-V // 8) * 8, device=h.device, dtype=torch.bfloat16)[:, :V]  # 16-byte rows
+        loss = torch.empty(M, device=h.device, dtype=torch.float32)
+        count, inv_n, total = _count(t, ids, V), _scalar(t), _scalar(t)
+        _reduce(None, count, None, inv_n)
+        for s0 in range(0, M, max(chunk, 1)):
+            rows = slice(s0, min(M, s0 + chunk))
+            gemm(h2[rows], w, trans_b=True, out=dlogits[rows])
+            _rows(dlogits[rows], t[rows], ids[rows], temperature, loss[rows], None, dlogits[rows], None, inv_n)
+        _reduce(loss, count, total, None)
+        ctx.save_for_backward(h2, w, dlogits)
+        ctx.hshape = h.shape
+        return total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        h2, w, dlogits = ctx.saved_tensors
+        alpha = float(g)  # scalar loss: fold the upstream gradient into the GEMM alpha
+        dh = gemm(dlogits, w, alpha=alpha).view(ctx.hshape) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.needs_input_grad[1]:
+            if has_main_grad(w):
+                gemm(dlogits, h2, trans_a=True, out=w.main_grad, beta=main_grad_beta(w), alpha=alpha)
+            else:
+                dw = gemm(dlogits, h2, trans_a=True, out_dtype=torch.float32, alpha=alpha).to(w.dtype)
+        return dh, dw, None, None, None, None
+
+
+def linear_topk_distillation(h, w, teacher_logits, teacher_ids, temperature: float = 1.0, chunk: int = 0):
+    """Mean :func:`topk_distillation` of the logits ``h @ w.T`` (h [..., D], w [V, D], bf16 on CUDA), with the
+    logits held once and turned into their gradient in place, optionally ``chunk`` tokens at a time."""
+    if h.shape[-1] != w.shape[-1] or w.dim() != 2 or h.dim() < 1:
+        raise ValueError(f"linear_topk_distillation: h {tuple(h.shape)}, w {tuple(w.shape)}")
+    if chunk < 0:
+        raise ValueError(f"linear_topk_distillation: chunk {chunk}")
+    _check("linear_topk_distillation", h, teacher_logits, teacher_ids, temperature, "mean")
+    same_device(h, w)
+    if not h.is_cuda:
+        logits = torch.nn.functional.linear(h.float(), w.float())
+        return topk_distillation_ref(logits, teacher_logits, teacher_ids, temperature)
+    for x in (h, w):
+        dtype_code("linear_topk_distillation", x, (torch.bfloat16,))
+    t, ids = _teacher(teacher_logits, teacher_ids)
+    return _LinearDistillFn.apply(h, w, t, ids, float(temperature), chunk)

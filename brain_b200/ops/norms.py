@@ -13,7 +13,8 @@ from __future__ import annotations
 import torch
 
 from .. import _native
-from ._common import has_main_grad, main_grad_beta, ptr, rows2d, stream
+from ._common import (dtype_code, has_main_grad, launch, main_grad_beta, no_backward, ptr, rows2d, same_device,
+                      stream)
 
 _RMS, _LN = 0, 1
 
@@ -157,3 +158,56 @@ def fused_layer_norm(x, w, b=None, eps=1e-5):
     if b is not None:
         y = y + b.to(ct)
     return y.to(x.dtype)
+
+
+# ------------------------------------------------------------------ e4m3 output (inference)
+def rms_norm_fp8_ref(s, w, eps, scaling):
+    y = s.float()
+    y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+    if scaling == "block":
+        y = y.view(*s.shape[:-1], s.shape[-1] // 128, 128)
+    amax = y.abs().amax(-1)
+    scale = torch.where(amax > 0, (amax / 448.0).clamp_min(2.0 ** -126), torch.ones_like(amax))
+    return (y / scale[..., None]).to(torch.float8_e4m3fn).view(s.shape), scale
+
+
+def _norm_fp8(name, x, r, w, eps, scaling):
+    if scaling not in ("rowwise", "block"):
+        raise ValueError(f"unknown fp8 scaling {scaling!r}")
+    D = x.shape[-1] if x.dim() else 0
+    if D == 0 or (scaling == "block" and D % 128):
+        raise ValueError(f"{name}: last dimension {D}" + (" is not a multiple of 128" if D else ""))
+    if w.shape != (D,) or (r is not None and r.shape != x.shape):
+        raise ValueError(f"{name}: x {tuple(x.shape)}, residual {None if r is None else tuple(r.shape)}, "
+                         f"weight {tuple(w.shape)}")
+    if w.dtype != x.dtype or (r is not None and r.dtype != x.dtype):
+        raise TypeError(f"{name}: x, the residual and the weight are of one type")
+    code = dtype_code(name, x)
+    no_backward(name, x, r, w)
+    same_device(x, r, w)
+    if not x.is_cuda:
+        s = x if r is None else (x.float() + r.float()).to(x.dtype)
+        return *rms_norm_fp8_ref(s, w, eps, scaling), s
+    x2 = rows2d(x)
+    M = x2.shape[0]
+    r2 = None if r is None else rows2d(r)
+    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    block = scaling == "block"
+    scale = torch.empty((*x.shape[:-1], D // 128) if block else x.shape[:-1], device=x.device, dtype=torch.float32)
+    s = None if r is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    launch(x, "brain_norm_fp8", code, x2.data_ptr(), x2.stride(0), ptr(r2), 0 if r2 is None else r2.stride(0),
+           w.contiguous().data_ptr(), ptr(s), q.data_ptr(), scale.data_ptr(), M, D, int(block), float(eps))
+    return q, scale, s
+
+
+def rms_norm_fp8(x, w, eps=1e-6, scaling: str = "rowwise"):
+    """``rms_norm(x, w)`` quantised to e4m3 in the same pass -> (q, scale), the operand that the fp8 GEMMs take
+    (``quantization.fp8_gemm_rowwise`` / ``fp8_gemm_blockscaled``): one scale a row (``"rowwise"``, scale of
+    x's leading shape) or one per 128 values (``"block"``, [..., D / 128]), amax / 448, at least 2^-126 (1 for
+    zeros). The norm is quantised from float32, without a rounding to x's type in between. Inference only."""
+    return _norm_fp8("rms_norm_fp8", x, None, w, eps, scaling)[:2]
+
+
+def add_rms_norm_fp8(x, r, w, eps=1e-6, scaling: str = "rowwise"):
+    """``add_rms_norm`` with the e4m3 output of :func:`rms_norm_fp8` -> (q, scale, x + r)."""
+    return _norm_fp8("add_rms_norm_fp8", x, r, w, eps, scaling)

@@ -3,7 +3,8 @@ quantisation (``BlockQuantizer``, block_quant.rs:20-70; int4 packing, dtype_map.
 linear layers with int32-style accumulation (``QLinear`` qlinear.rs:26-110, ``q8_matmul``
 qmatmul.rs:34-66), calibration observers, SmoothQuant scales (act_quant.rs:47-74), fake quantisation
 with a straight-through estimator, magnitude pruning, and the FP8 E4M3 **1x128 block-scaled** format
-(declared but without math in the reference) used by the sm_100a FP8 GEMM (``csrc/fp8.cu``).
+(declared but without math in the reference) used by the sm_100a FP8 GEMM (``csrc/fp8.cu``), and 4-bit weights
+with group scales and their product with a few tokens (``csrc/int4.cu``).
 """
 from __future__ import annotations
 
@@ -13,6 +14,7 @@ import torch
 
 from .fp8 import (dequantize_fp8_blockwise, fp8_linear, fp8_gemm_blockscaled, quantize_fp8_blockwise,  # noqa: F401
                   quantize_fp8_weight_blocks, quantize_fp8_rowwise, fp8_gemm_rowwise, fp8_linear_rowwise, Fp8Linear)
+from .int4 import Int4Linear, dequantize_int4, int4_linear, quantize_int4  # noqa: F401
 
 
 class QuantDType(enum.Enum):
