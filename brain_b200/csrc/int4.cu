@@ -6,13 +6,26 @@
 // a group's sum is multiplied by its scale in f32, and y is rounded once.
 //
 // Bound by memory: N K / 2 bytes of weights and their scales, read once for all tokens of a call.
+//
+// The tensor cores' warp-level 16 x 8 x 16 product takes 16 output rows of the weight as its rows and 8
+// tokens as its columns, so one to eight tokens cost the same. Its operand order along K is free as long as
+// both sides agree: a lane takes the 8 values of one 32-bit word of its row at a time, the pairs (i, i + 4)
+// that a shift and a mask leave in the two halves of a register, and pairs the activations alike. Masked
+// onto the exponent bits of 128 (bf16) or 1024 (f16) a nibble is that number plus its value; one packed
+// subtraction takes the base and the zero point off, exactly.
+//
+// A CTA owns 16 RT output rows, its 8 warps split K in pairs of 128-wide chunks. Weights and activations of a
+// chunk come through a ring of asynchronous copies that each warp runs for itself (no block barrier in the
+// loop, as many bytes in flight as shared memory holds); the scales of a chunk are requested when its copies
+// are. The warps' sums meet in shared memory in a fixed order.
 #include "elem.cuh"
 
 using namespace brain;
 
 namespace {
 
-constexpr int kTok = 8;  // tokens a pass
+constexpr int kWarps = 8;
+constexpr int kChunk = 128;  // K of one ring stage: 64 bytes of a weight row
 
 struct Int4Args {
   const void* x;      // [M, K]
@@ -26,59 +39,240 @@ struct Int4Args {
   int M, N, K, G, groups;
 };
 
-// One warp per output row and 8 tokens; a lane takes 8 values (one word) at a time.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where !on
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) int4_kernel(Int4Args a) {
-  const int n = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int m0 = blockIdx.y * kTok, mt = min(kTok, a.M - m0);
-  if (n >= a.N) return;
-  const uint8_t* w = a.w + n * a.ldw;
-  const T* s = (const T*)a.s + (int64_t)n * a.groups;
-  float acc[kTok] = {};
-  for (int k = lane * 8; k < a.K; k += 256) {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(w + k / 2);
-    const int g = k / a.G;
-    const float sc = to_f32(s[g]);
-    const int zero = a.z ? a.z[(int64_t)n * a.groups + g] : 0;
-    float f[8];
+struct Half2;  // the pair type, its exponent base and the product
+template <>
+struct Half2<__nv_bfloat16> {
+  static constexpr uint32_t kBase = 0x43004300u;  // 128, 128
+  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Half2<__half> {
+  static constexpr uint32_t kBase = 0x64006400u;  // 1024, 1024
+  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+// Pair i of a word of 8 values: (value i, value i + 4) as T; `flip` turns two's complement into an offset of 8.
+template <typename T>
+__device__ __forceinline__ uint32_t unpack(uint32_t w, int i, uint32_t magic, uint32_t off) {
+  return Half2<T>::sub(((w >> (4 * i)) & 0x000f000fu) ^ magic, off);
+}
+
+// RT: 16-row tiles a CTA; NT: 8-token tiles; FL: scales a row and chunk (128 / G, at least 1); S: ring stages.
+template <typename T, int RT, int NT, int FL, int S>
+__global__ void __launch_bounds__(kWarps * 32) int4_kernel(Int4Args a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
+  const int n0 = blockIdx.x * 16 * RT, m0 = blockIdx.y * 8 * NT, mt = min(8 * NT, a.M - m0);
+  const int stage_bytes = RT * 1024 + mt * 256;
+  const uint32_t ring = smem_u32(smem) + warp * S * stage_bytes;
+  const int chunks = (a.K + kChunk - 1) / kChunk;
+  // chunk pairs (a 128-byte line of every row) go round the warps
+  const int whole = chunks / (2 * kWarps), rest = min(max(chunks - whole * 2 * kWarps - 2 * warp, 0), 2);
+  const int mine = 2 * whole + rest;
+  const T* x = (const T*)a.x + m0 * a.ldx;
+  const T* scale = (const T*)a.s;
+  const uint32_t magic = a.z ? Half2<T>::kBase : Half2<T>::kBase ^ 0x00080008u;
+
+  const uint8_t* wrow[RT][2];
+  int64_t srow[RT][2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int nib = (v >> (4 * j)) & 15;
-      f[j] = (float)(a.z ? nib - zero : (nib ^ 8) - 8);
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int n = min(n0 + r * 16 + h * 8 + g, a.N - 1);  // rows past the end repeat the last, and are not stored
+      wrow[r][h] = a.w + n * a.ldw + t4 * 16;
+      srow[r][h] = (int64_t)n * a.groups;
     }
+  const uint32_t wdst = g * 64 + ((t4 ^ ((g >> 1) & 3)) * 16);
+
+  // the scales (and zero points) of the chunks in the ring
+  T sc[S][RT][2][FL];
+  uint8_t zp[S][RT][2][FL];
+  auto fetch = [&](int it, int st) {
+    if (it < mine) {
+      const int k0 = (((it >> 1) * kWarps + warp) * 2 + (it & 1)) * kChunk;
+      const uint32_t dst = ring + st * stage_bytes;
+      const bool on = k0 + t4 * 32 < a.K;
 #pragma unroll
-    for (int m = 0; m < kTok; ++m)
-      if (m < mt) {
-        const T* x = (const T*)a.x + (m0 + m) * a.ldx + k;
-        float d = 0.f;
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d = fmaf(to_f32(x[j]), f[j], d);
-        acc[m] = fmaf(d, sc, acc[m]);
+        for (int h = 0; h < 2; ++h)
+          copy16(dst + r * 1024 + h * 512 + wdst, on ? wrow[r][h] + k0 / 2 : a.w, on);
+      const int j = g & 3;
+      const bool xon = k0 + j * 32 < a.K;
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) {
+        const int tok = lane / 16 + 2 * i;
+        if (tok < mt)
+          copy16(dst + RT * 1024 + tok * 256 + ((j ^ (tok & 3)) * 64) + t4 * 16,
+                 xon ? x + tok * a.ldx + k0 + (lane & 15) * 8 : a.x, xon);
       }
-  }
 #pragma unroll
-  for (int m = 0; m < kTok; ++m) {
-    const float v = warp_sum(acc[m]);
-    if (lane == 0 && m < mt)
-      ((T*)a.y)[(int64_t)(m0 + m) * a.N + n] = from_f32<T>(v + (a.bias ? to_f32(((const T*)a.bias)[n]) : 0.f));
+      for (int f = 0; f < FL; ++f) {
+        const int grp = min((k0 + f * (kChunk / FL)) / a.G, a.groups - 1);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            sc[st][r][h][f] = scale[srow[r][h] + grp];
+            if (a.z) zp[st][r][h][f] = a.z[srow[r][h] + grp];
+          }
+      }
+    }
+    copy_commit();
+  };
+
+  float sum[RT][NT][4] = {};
+#pragma unroll
+  for (int st = 0; st < S - 1; ++st) fetch(st, st);
+  for (int it0 = 0; it0 < mine; it0 += S) {
+#pragma unroll
+    for (int st = 0; st < S; ++st) {
+      const int it = it0 + st;
+      if (it < mine) {
+        copy_wait<S - 2>();
+        __syncwarp();
+        fetch(it + S - 1, (st + S - 1) % S);
+        const uint8_t* at = smem + warp * S * stage_bytes + st * stage_bytes;
+        const uint8_t* xs = at + RT * 1024;
+        float acc[RT][NT][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t b[NT][4];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const int tok = min(t * 8 + g, mt - 1);  // columns past the last token are not stored
+            const uint4 v = *reinterpret_cast<const uint4*>(xs + tok * 256 + ((j ^ (tok & 3)) * 64) + t4 * 16);
+            b[t][0] = __byte_perm(v.x, v.z, 0x5410);
+            b[t][1] = __byte_perm(v.x, v.z, 0x7632);
+            b[t][2] = __byte_perm(v.y, v.w, 0x5410);
+            b[t][3] = __byte_perm(v.y, v.w, 0x7632);
+          }
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            uint32_t off[2], q[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              off[h] = a.z ? Half2<T>::kBase + zp[st][r][h][j * FL / 4] * 0x00010001u : magic;
+              const uint32_t word = *reinterpret_cast<const uint32_t*>(at + r * 1024 + h * 512 + g * 64 +
+                                                                       ((j ^ ((g >> 1) & 3)) * 16) + t4 * 4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) q[h][i] = unpack<T>(word, i, magic, off[h]);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              Half2<T>::mma(acc[r][t], q[0][0], q[1][0], q[0][1], q[1][1], b[t][0], b[t][1]);
+              Half2<T>::mma(acc[r][t], q[0][2], q[1][2], q[0][3], q[1][3], b[t][2], b[t][3]);
+            }
+            if ((j + 1) % (4 / FL) == 0) {  // the end of a group, or of the chunk in a wider one
+              const float s0 = to_f32(sc[st][r][0][j * FL / 4]), s1 = to_f32(sc[st][r][1][j * FL / 4]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                sum[r][t][0] = fmaf(s0, acc[r][t][0], sum[r][t][0]);
+                sum[r][t][1] = fmaf(s0, acc[r][t][1], sum[r][t][1]);
+                sum[r][t][2] = fmaf(s1, acc[r][t][2], sum[r][t][2]);
+                sum[r][t][3] = fmaf(s1, acc[r][t][3], sum[r][t][3]);
+                acc[r][t][0] = acc[r][t][1] = acc[r][t][2] = acc[r][t][3] = 0.f;
+              }
+            }
+          }
+        }
+      }
+    }
   }
+  copy_wait<0>();
+  __syncthreads();
+  // [warp][token][row] partial sums over the ring's place
+  constexpr int kRows = 16 * RT;
+  float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int tok = t * 8 + t4 * 2 + (c & 1), row = r * 16 + (c / 2) * 8 + g;
+        if (tok < mt) part[(warp * mt + tok) * kRows + row] = sum[r][t][c];
+      }
+  __syncthreads();
+  for (int i = threadIdx.x; i < mt * kRows; i += kWarps * 32) {
+    const int n = n0 + i % kRows;
+    if (n >= a.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) v += part[k * mt * kRows + i];
+    if (a.bias) v += to_f32(((const T*)a.bias)[n]);
+    ((T*)a.y)[(int64_t)(m0 + i / kRows) * a.N + n] = from_f32<T>(v);
+  }
+}
+
+template <typename T, int RT, int NT, int FL, int S>
+int launch_ring(const Int4Args& a, cudaStream_t st) {
+  const int mt = a.M < 8 * NT ? a.M : 8 * NT;
+  const int ring = kWarps * S * (RT * 1024 + mt * 256), part = kWarps * mt * 16 * RT * 4;
+  const int smem = ring > part ? ring : part;
+  static const cudaError_t e =
+      cudaFuncSetAttribute(int4_kernel<T, RT, NT, FL, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e != cudaSuccess) return (int)e;
+  const dim3 grid((a.N + 16 * RT - 1) / (16 * RT), (a.M + 8 * NT - 1) / (8 * NT));
+  int4_kernel<T, RT, NT, FL, S><<<grid, kWarps * 32, smem, st>>>(a);
+  return (int)cudaGetLastError();
+}
+
+template <typename T, int FL>
+int launch_tokens(const Int4Args& a, cudaStream_t st) {
+  if (a.M <= 8) return launch_ring<T, 2, 1, FL, 4>(a, st);
+  if (a.M <= 16) return launch_ring<T, 2, 2, FL, 2>(a, st);
+  return launch_ring<T, 2, 4, FL, 2>(a, st);
 }
 
 template <typename T>
 int launch(const Int4Args& a, cudaStream_t st) {
-  const dim3 grid((a.N + 7) / 8, (a.M + kTok - 1) / kTok);
-  int4_kernel<T><<<grid, 256, 0, st>>>(a);
-  return (int)cudaGetLastError();
+  // a scale may change inside a chunk: every 32 or 64 values, or at a multiple of 32 that is neither
+  if (a.G % kChunk == 0) return launch_tokens<T, 1>(a, st);
+  if (a.G % 64 == 0) return launch_tokens<T, 2>(a, st);
+  return launch_tokens<T, 4>(a, st);
 }
 
 }  // namespace
 
-// K and G multiples of 32, groups = ceil(K / G); w rows 16-byte aligned; y [M, N] contiguous.
+// K and G multiples of 32, groups = ceil(K / G); w and x rows 16-byte aligned; y [M, N] contiguous.
 BRAIN_API int brain_int4_linear(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* s,
                                 const void* z, const void* bias, void* y, int M, int N, int K, int G,
                                 cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || K % 32 || G <= 0 || G % 32 || ldw % 16 || ((uintptr_t)w & 15) || M > 8 * 65535)
+  if (K <= 0 || K % 32 || G <= 0 || G % 32 || ldw % 16 || ((uintptr_t)w & 15) || ldx % 8 || ((uintptr_t)x & 15) ||
+      M > 8 * 65535)
     return (int)cudaErrorInvalidValue;
   const Int4Args a{x, ldx, (const uint8_t*)w, ldw, s, (const uint8_t*)z, bias, y, M, N, K, G, (K + G - 1) / G};
   switch (dtype) {

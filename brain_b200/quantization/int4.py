@@ -94,6 +94,8 @@ def int4_linear(x, packed, scales, zeros=None, bias=None, group_size: int = 128)
     if packed.stride(1) != 1 or packed.stride(0) % 16 or packed.data_ptr() % 16:
         raise ValueError("int4_linear: the packed weight's rows have to be adjacent bytes that start on 16 bytes")
     x2 = rows2d(x)
+    if x2.stride(0) % 8 or x2.data_ptr() % 16:  # the kernel copies 16 bytes at a time
+        x2 = x2.clone(memory_format=torch.contiguous_format)
     y = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
     launch(x, "brain_int4_linear", code, x2.data_ptr(), x2.stride(0), packed.data_ptr(), packed.stride(0),
            scales.contiguous().data_ptr(), None if zeros is None else zeros.contiguous().data_ptr(), ptr(bias),
