@@ -36,7 +36,10 @@ struct Int4Args {
   const uint8_t* z;   // [N, groups] or null
   const void* bias;   // [N] or null
   void* y;            // [M, N]
-  int M, N, K, G, groups;
+  int M, N, K, groups;
+  // k / G of a k that 32 divides is the high half of (k / 32) inv_g, inv_g the next whole number above
+  // 2^32 / (G / 32): exact while (k / 32) (G / 32) < 2^32, and G <= K <= 2^20. 0: G is 32
+  uint32_t inv_g;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where !on
@@ -81,130 +84,154 @@ struct Half2<__half> {
   }
 };
 
-// Pair i of a word of 8 values: (value i, value i + 4) as T; `flip` turns two's complement into an offset of 8.
+// Pair i of a word of 8 values: (value i, value i + 4) less the offset that `off` holds, as T. `magic` is the
+// base's exponent, with bit 3 set where the values are two's complement (which makes them an offset of 8).
 template <typename T>
 __device__ __forceinline__ uint32_t unpack(uint32_t w, int i, uint32_t magic, uint32_t off) {
   return Half2<T>::sub(((w >> (4 * i)) & 0x000f000fu) ^ magic, off);
 }
 
-// RT: 16-row tiles a CTA; NT: 8-token tiles; FL: scales a row and chunk (128 / G, at least 1); S: ring stages.
-template <typename T, int RT, int NT, int FL, int S>
-__global__ void __launch_bounds__(kWarps * 32) int4_kernel(Int4Args a) {
+__device__ __forceinline__ uint32_t group_of(uint32_t k32, uint32_t inv_g) {
+  return inv_g ? __umulhi(k32, inv_g) : k32;
+}
+
+// RT: 16-row tiles a CTA; NT: 8-token tiles; FL: scales a row and chunk (128 / G, at least 1); ZP: zero points;
+// S: ring stages.
+template <typename T, int RT, int NT, int FL, bool ZP, int S>
+__global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ? 3 : 2) int4_kernel(Int4Args a) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
   const int n0 = blockIdx.x * 16 * RT, m0 = blockIdx.y * 8 * NT, mt = min(8 * NT, a.M - m0);
-  const int stage_bytes = RT * 1024 + mt * 256;
-  const uint32_t ring = smem_u32(smem) + warp * S * stage_bytes;
+  const uint32_t stage_bytes = RT * 1024 + mt * 256;
+  const uint8_t* ring = smem + warp * S * stage_bytes;
   const int chunks = (a.K + kChunk - 1) / kChunk;
   // chunk pairs (a 128-byte line of every row) go round the warps
   const int whole = chunks / (2 * kWarps), rest = min(max(chunks - whole * 2 * kWarps - 2 * warp, 0), 2);
   const int mine = 2 * whole + rest;
-  const T* x = (const T*)a.x + m0 * a.ldx;
-  const T* scale = (const T*)a.s;
-  const uint32_t magic = a.z ? Half2<T>::kBase : Half2<T>::kBase ^ 0x00080008u;
+  constexpr uint32_t magic = ZP ? Half2<T>::kBase : Half2<T>::kBase ^ 0x00080008u;
 
-  const uint8_t* wrow[RT][2];
-  int64_t srow[RT][2];
+  // one base for the CTA, 32-bit offsets for its lanes; rows past the end repeat the last, and are not stored
+  const uint8_t* wbase = a.w + n0 * a.ldw;
+  const T* sbase = (const T*)a.s + (int64_t)n0 * a.groups;
+  const uint8_t* zbase = ZP ? a.z + (int64_t)n0 * a.groups : nullptr;
+  const uint8_t* xbase = (const uint8_t*)a.x + m0 * a.ldx * 2;
+  uint32_t woff[RT][2], soff[RT][2];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int n = min(n0 + r * 16 + h * 8 + g, a.N - 1);  // rows past the end repeat the last, and are not stored
-      wrow[r][h] = a.w + n * a.ldw + t4 * 16;
-      srow[r][h] = (int64_t)n * a.groups;
+      const uint32_t n = min(r * 16 + h * 8 + g, a.N - 1 - n0);
+      woff[r][h] = n * (uint32_t)a.ldw;
+      soff[r][h] = n * a.groups;
     }
-  const uint32_t wdst = g * 64 + ((t4 ^ ((g >> 1) & 3)) * 16);
+  const uint32_t wdst = smem_u32(ring) + g * 64 + ((t4 ^ ((g >> 1) & 3)) * 16);
+  const uint32_t xdst = smem_u32(ring) + RT * 1024 + (lane / 16) * 256 + t4 * 16;
+  const uint32_t xoff = (lane / 16) * (uint32_t)a.ldx * 2;
 
-  // the scales (and zero points) of the chunks in the ring
-  T sc[S][RT][2][FL];
-  uint8_t zp[S][RT][2][FL];
+  auto first_k = [&](int it) { return (((it >> 1) * kWarps + warp) * 2 + (it & 1)) * kChunk; };
   auto fetch = [&](int it, int st) {
     if (it < mine) {
-      const int k0 = (((it >> 1) * kWarps + warp) * 2 + (it & 1)) * kChunk;
-      const uint32_t dst = ring + st * stage_bytes;
+      const int k0 = first_k(it);
+      const uint32_t stage = st * stage_bytes;
       const bool on = k0 + t4 * 32 < a.K;
+      const uint32_t kw = on ? k0 / 2 + t4 * 16 : 0;
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          copy16(dst + r * 1024 + h * 512 + wdst, on ? wrow[r][h] + k0 / 2 : a.w, on);
+        for (int h = 0; h < 2; ++h) copy16(wdst + stage + r * 1024 + h * 512, wbase + (woff[r][h] + kw), on);
       const int j = g & 3;
       const bool xon = k0 + j * 32 < a.K;
+      const uint32_t kx = xon ? xoff + (k0 + (lane & 15) * 8) * 2 : 0;
 #pragma unroll
       for (int i = 0; i < 4 * NT; ++i) {
         const int tok = lane / 16 + 2 * i;
         if (tok < mt)
-          copy16(dst + RT * 1024 + tok * 256 + ((j ^ (tok & 3)) * 64) + t4 * 16,
-                 xon ? x + tok * a.ldx + k0 + (lane & 15) * 8 : a.x, xon);
+          copy16(xdst + stage + i * 512 + ((j ^ (tok & 3)) * 64), xbase + (kx + (xon ? i * (uint32_t)a.ldx * 4 : 0)), xon);
       }
+    }
+    copy_commit();
+  };
+  // the scales (and zero points) of a chunk, asked for one chunk ahead
+  T sc[RT][2][FL], scn[RT][2][FL];
+  uint8_t zp[RT][2][FL], zpn[RT][2][FL];
+  auto scales = [&](int it) {
+    if (it < mine) {
+      const uint32_t k32 = first_k(it) / 32;
 #pragma unroll
       for (int f = 0; f < FL; ++f) {
-        const int grp = min((k0 + f * (kChunk / FL)) / a.G, a.groups - 1);
+        const uint32_t grp = min((int)group_of(k32 + f * (4 / FL), a.inv_g), a.groups - 1);
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            sc[st][r][h][f] = scale[srow[r][h] + grp];
-            if (a.z) zp[st][r][h][f] = a.z[srow[r][h] + grp];
+            scn[r][h][f] = sbase[soff[r][h] + grp];
+            if (ZP) zpn[r][h][f] = zbase[soff[r][h] + grp];
           }
       }
     }
-    copy_commit();
   };
 
   float sum[RT][NT][4] = {};
 #pragma unroll
   for (int st = 0; st < S - 1; ++st) fetch(st, st);
-  for (int it0 = 0; it0 < mine; it0 += S) {
+  scales(0);
+  int st = 0;
+#pragma unroll 1
+  for (int it = 0; it < mine; ++it) {
+    copy_wait<S - 2>();
+    __syncwarp();
+    fetch(it + S - 1, st == 0 ? S - 1 : st - 1);
 #pragma unroll
-    for (int st = 0; st < S; ++st) {
-      const int it = it0 + st;
-      if (it < mine) {
-        copy_wait<S - 2>();
-        __syncwarp();
-        fetch(it + S - 1, (st + S - 1) % S);
-        const uint8_t* at = smem + warp * S * stage_bytes + st * stage_bytes;
-        const uint8_t* xs = at + RT * 1024;
-        float acc[RT][NT][4] = {};
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t b[NT][4];
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int f = 0; f < FL; ++f) {
+          sc[r][h][f] = scn[r][h][f];
+          if (ZP) zp[r][h][f] = zpn[r][h][f];
+        }
+    scales(it + 1);
+    const uint8_t* at = ring + st * stage_bytes + g * 64 + t4 * 4;
+    const uint8_t* xs = ring + st * stage_bytes + RT * 1024 + t4 * 16;
+    st = st == S - 1 ? 0 : st + 1;
+    float acc[RT][NT][4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t b[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int tok = min(t * 8 + g, mt - 1);  // columns past the last token are not stored
+        const uint4 v = *reinterpret_cast<const uint4*>(xs + tok * 256 + ((j ^ (tok & 3)) * 64));
+        b[t][0] = __byte_perm(v.x, v.z, 0x5410);
+        b[t][1] = __byte_perm(v.x, v.z, 0x7632);
+        b[t][2] = __byte_perm(v.y, v.w, 0x5410);
+        b[t][3] = __byte_perm(v.y, v.w, 0x7632);
+      }
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        uint32_t q[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t off = ZP ? Half2<T>::kBase + zp[r][h][j * FL / 4] * 0x00010001u : magic;
+          const uint32_t word =
+              *reinterpret_cast<const uint32_t*>(at + r * 1024 + h * 512 + ((j ^ ((g >> 1) & 3)) * 16));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[h][i] = unpack<T>(word, i, magic, off);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          Half2<T>::mma(acc[r][t], q[0][0], q[1][0], q[0][1], q[1][1], b[t][0], b[t][1]);
+          Half2<T>::mma(acc[r][t], q[0][2], q[1][2], q[0][3], q[1][3], b[t][2], b[t][3]);
+        }
+        if ((j + 1) % (4 / FL) == 0) {  // the end of a group, or of the chunk in a wider one
+          const float s0 = to_f32(sc[r][0][j * FL / 4]), s1 = to_f32(sc[r][1][j * FL / 4]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const int tok = min(t * 8 + g, mt - 1);  // columns past the last token are not stored
-            const uint4 v = *reinterpret_cast<const uint4*>(xs + tok * 256 + ((j ^ (tok & 3)) * 64) + t4 * 16);
-            b[t][0] = __byte_perm(v.x, v.z, 0x5410);
-            b[t][1] = __byte_perm(v.x, v.z, 0x7632);
-            b[t][2] = __byte_perm(v.y, v.w, 0x5410);
-            b[t][3] = __byte_perm(v.y, v.w, 0x7632);
-          }
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            uint32_t off[2], q[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              off[h] = a.z ? Half2<T>::kBase + zp[st][r][h][j * FL / 4] * 0x00010001u : magic;
-              const uint32_t word = *reinterpret_cast<const uint32_t*>(at + r * 1024 + h * 512 + g * 64 +
-                                                                       ((j ^ ((g >> 1) & 3)) * 16) + t4 * 4);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) q[h][i] = unpack<T>(word, i, magic, off[h]);
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              Half2<T>::mma(acc[r][t], q[0][0], q[1][0], q[0][1], q[1][1], b[t][0], b[t][1]);
-              Half2<T>::mma(acc[r][t], q[0][2], q[1][2], q[0][3], q[1][3], b[t][2], b[t][3]);
-            }
-            if ((j + 1) % (4 / FL) == 0) {  // the end of a group, or of the chunk in a wider one
-              const float s0 = to_f32(sc[st][r][0][j * FL / 4]), s1 = to_f32(sc[st][r][1][j * FL / 4]);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                sum[r][t][0] = fmaf(s0, acc[r][t][0], sum[r][t][0]);
-                sum[r][t][1] = fmaf(s0, acc[r][t][1], sum[r][t][1]);
-                sum[r][t][2] = fmaf(s1, acc[r][t][2], sum[r][t][2]);
-                sum[r][t][3] = fmaf(s1, acc[r][t][3], sum[r][t][3]);
-                acc[r][t][0] = acc[r][t][1] = acc[r][t][2] = acc[r][t][3] = 0.f;
-              }
-            }
+            sum[r][t][0] = fmaf(s0, acc[r][t][0], sum[r][t][0]);
+            sum[r][t][1] = fmaf(s0, acc[r][t][1], sum[r][t][1]);
+            sum[r][t][2] = fmaf(s1, acc[r][t][2], sum[r][t][2]);
+            sum[r][t][3] = fmaf(s1, acc[r][t][3], sum[r][t][3]);
+            acc[r][t][0] = acc[r][t][1] = acc[r][t][2] = acc[r][t][3] = 0.f;
           }
         }
       }
@@ -236,32 +263,37 @@ __global__ void __launch_bounds__(kWarps * 32) int4_kernel(Int4Args a) {
   }
 }
 
-template <typename T, int RT, int NT, int FL, int S>
+template <typename T, int RT, int NT, int FL, bool ZP, int S>
 int launch_ring(const Int4Args& a, cudaStream_t st) {
   const int mt = a.M < 8 * NT ? a.M : 8 * NT;
   const int ring = kWarps * S * (RT * 1024 + mt * 256), part = kWarps * mt * 16 * RT * 4;
   const int smem = ring > part ? ring : part;
-  static const cudaError_t e =
-      cudaFuncSetAttribute(int4_kernel<T, RT, NT, FL, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  const auto kernel = int4_kernel<T, RT, NT, FL, ZP, S>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
   const dim3 grid((a.N + 16 * RT - 1) / (16 * RT), (a.M + 8 * NT - 1) / (8 * NT));
-  int4_kernel<T, RT, NT, FL, S><<<grid, kWarps * 32, smem, st>>>(a);
+  kernel<<<grid, kWarps * 32, smem, st>>>(a);
   return (int)cudaGetLastError();
 }
 
-template <typename T, int FL>
+template <typename T, int FL, bool ZP>
 int launch_tokens(const Int4Args& a, cudaStream_t st) {
-  if (a.M <= 8) return launch_ring<T, 2, 1, FL, 4>(a, st);
-  if (a.M <= 16) return launch_ring<T, 2, 2, FL, 2>(a, st);
-  return launch_ring<T, 2, 4, FL, 2>(a, st);
+  if (a.M <= 8) return launch_ring<T, 2, 1, FL, ZP, 3>(a, st);
+  if (a.M <= 16) return launch_ring<T, 2, 2, FL, ZP, 2>(a, st);
+  return launch_ring<T, 2, 4, FL, ZP, 2>(a, st);
+}
+
+template <typename T, bool ZP>
+int launch_groups(const Int4Args& a, int G, cudaStream_t st) {
+  // a scale may change inside a chunk: every 64 values, or at any multiple of 32
+  if (G % kChunk == 0) return launch_tokens<T, 1, ZP>(a, st);
+  if (G % 64 == 0) return launch_tokens<T, 2, ZP>(a, st);
+  return launch_tokens<T, 4, ZP>(a, st);
 }
 
 template <typename T>
-int launch(const Int4Args& a, cudaStream_t st) {
-  // a scale may change inside a chunk: every 32 or 64 values, or at a multiple of 32 that is neither
-  if (a.G % kChunk == 0) return launch_tokens<T, 1>(a, st);
-  if (a.G % 64 == 0) return launch_tokens<T, 2>(a, st);
-  return launch_tokens<T, 4>(a, st);
+int launch(const Int4Args& a, int G, cudaStream_t st) {
+  return a.z ? launch_groups<T, true>(a, G, st) : launch_groups<T, false>(a, G, st);
 }
 
 }  // namespace
@@ -272,12 +304,14 @@ BRAIN_API int brain_int4_linear(int dtype, const void* x, int64_t ldx, const voi
                                 cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0 || K % 32 || G <= 0 || G % 32 || ldw % 16 || ((uintptr_t)w & 15) || ldx % 8 || ((uintptr_t)x & 15) ||
-      M > 8 * 65535)
+      M > 8 * 65535 || K > (1 << 20) || ldw > (1 << 26) || ldx > (1 << 26))
     return (int)cudaErrorInvalidValue;
-  const Int4Args a{x, ldx, (const uint8_t*)w, ldw, s, (const uint8_t*)z, bias, y, M, N, K, G, (K + G - 1) / G};
+  if (G > K) G = K;
+  const uint32_t inv_g = G == 32 ? 0 : (uint32_t)((1ull << 32) / (G / 32)) + 1;
+  const Int4Args a{x, ldx, (const uint8_t*)w, ldw, s, (const uint8_t*)z, bias, y, M, N, K, (K + G - 1) / G, inv_g};
   switch (dtype) {
-    case BRAIN_BF16: return launch<__nv_bfloat16>(a, st);
-    case BRAIN_F16: return launch<__half>(a, st);
+    case BRAIN_BF16: return launch<__nv_bfloat16>(a, G, st);
+    case BRAIN_F16: return launch<__half>(a, G, st);
   }
   return (int)cudaErrorInvalidValue;
 }
