@@ -25,7 +25,9 @@ using namespace brain;
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kChunk = 128;  // K of one ring stage: 64 bytes of a weight row
+constexpr int kChunk = 128;  // K of one ring stage: 64 bytes of a weight row, 256 of a token
+// rows in the ring: 64 + 16 and 256 + 64 bytes put the 8 rows (tokens) that a warp reads at once on other banks
+constexpr int kRow = 80, kTile = 16 * kRow, kTok = 320;
 
 struct Int4Args {
   const void* x;      // [M, K]
@@ -87,8 +89,10 @@ struct Half2<__half> {
 // Pair i of a word of 8 values: (value i, value i + 4) less the offset that `off` holds, as T. `magic` is the
 // base's exponent, with bit 3 set where the values are two's complement (which makes them an offset of 8).
 template <typename T>
-__device__ __forceinline__ uint32_t unpack(uint32_t w, int i, uint32_t magic, uint32_t off) {
-  return Half2<T>::sub(((w >> (4 * i)) & 0x000f000fu) ^ magic, off);
+__device__ __forceinline__ uint32_t unpack(uint32_t w, int i, uint32_t mask, uint32_t magic, uint32_t off) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(v) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));  // (w & mask) ^ magic
+  return Half2<T>::sub(v, off);
 }
 
 __device__ __forceinline__ uint32_t group_of(uint32_t k32, uint32_t inv_g) {
@@ -102,13 +106,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ?
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
   const int n0 = blockIdx.x * 16 * RT, m0 = blockIdx.y * 8 * NT, mt = min(8 * NT, a.M - m0);
-  const uint32_t stage_bytes = RT * 1024 + mt * 256;
+  const uint32_t stage_bytes = RT * kTile + mt * kTok;
   const uint8_t* ring = smem + warp * S * stage_bytes;
   const int chunks = (a.K + kChunk - 1) / kChunk;
   // chunk pairs (a 128-byte line of every row) go round the warps
   const int whole = chunks / (2 * kWarps), rest = min(max(chunks - whole * 2 * kWarps - 2 * warp, 0), 2);
   const int mine = 2 * whole + rest;
-  constexpr uint32_t magic = ZP ? Half2<T>::kBase : Half2<T>::kBase ^ 0x00080008u;
+  // in registers, so that one three-input operation masks a pair and sets its exponent
+  uint32_t mask, magic;
+  asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
+  asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(ZP ? Half2<T>::kBase : Half2<T>::kBase ^ 0x00080008u));
 
   // one base for the CTA, 32-bit offsets for its lanes; rows past the end repeat the last, and are not stored
   const uint8_t* wbase = a.w + n0 * a.ldw;
@@ -124,8 +131,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ?
       woff[r][h] = n * (uint32_t)a.ldw;
       soff[r][h] = n * a.groups;
     }
-  const uint32_t wdst = smem_u32(ring) + g * 64 + ((t4 ^ ((g >> 1) & 3)) * 16);
-  const uint32_t xdst = smem_u32(ring) + RT * 1024 + (lane / 16) * 256 + t4 * 16;
+  const uint32_t wdst = smem_u32(ring) + g * kRow + t4 * 16;
+  const uint32_t xdst = smem_u32(ring) + RT * kTile + (lane / 16) * kTok + (lane & 15) * 16;
   const uint32_t xoff = (lane / 16) * (uint32_t)a.ldx * 2;
 
   auto first_k = [&](int it) { return (((it >> 1) * kWarps + warp) * 2 + (it & 1)) * kChunk; };
@@ -138,15 +145,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ?
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) copy16(wdst + stage + r * 1024 + h * 512, wbase + (woff[r][h] + kw), on);
-      const int j = g & 3;
-      const bool xon = k0 + j * 32 < a.K;
+        for (int h = 0; h < 2; ++h) copy16(wdst + stage + r * kTile + h * 8 * kRow, wbase + (woff[r][h] + kw), on);
+      const bool xon = k0 + (g & 3) * 32 < a.K;
       const uint32_t kx = xon ? xoff + (k0 + (lane & 15) * 8) * 2 : 0;
 #pragma unroll
       for (int i = 0; i < 4 * NT; ++i) {
         const int tok = lane / 16 + 2 * i;
         if (tok < mt)
-          copy16(xdst + stage + i * 512 + ((j ^ (tok & 3)) * 64), xbase + (kx + (xon ? i * (uint32_t)a.ldx * 4 : 0)), xon);
+          copy16(xdst + stage + i * 2 * kTok, xbase + (kx + (xon ? i * (uint32_t)a.ldx * 4 : 0)), xon);
       }
     }
     copy_commit();
@@ -191,8 +197,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ?
           if (ZP) zp[r][h][f] = zpn[r][h][f];
         }
     scales(it + 1);
-    const uint8_t* at = ring + st * stage_bytes + g * 64 + t4 * 4;
-    const uint8_t* xs = ring + st * stage_bytes + RT * 1024 + t4 * 16;
+    const uint8_t* at = ring + st * stage_bytes + g * kRow + t4 * 4;
+    const uint8_t* xs = ring + st * stage_bytes + RT * kTile + t4 * 16;
     st = st == S - 1 ? 0 : st + 1;
     float acc[RT][NT][4] = {};
 #pragma unroll
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ?
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int tok = min(t * 8 + g, mt - 1);  // columns past the last token are not stored
-        const uint4 v = *reinterpret_cast<const uint4*>(xs + tok * 256 + ((j ^ (tok & 3)) * 64));
+        const uint4 v = *reinterpret_cast<const uint4*>(xs + tok * kTok + j * 64);
         b[t][0] = __byte_perm(v.x, v.z, 0x5410);
         b[t][1] = __byte_perm(v.x, v.z, 0x7632);
         b[t][2] = __byte_perm(v.y, v.w, 0x5410);
@@ -214,9 +220,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ?
         for (int h = 0; h < 2; ++h) {
           const uint32_t off = ZP ? Half2<T>::kBase + zp[r][h][j * FL / 4] * 0x00010001u : magic;
           const uint32_t word =
-              *reinterpret_cast<const uint32_t*>(at + r * 1024 + h * 512 + ((j ^ ((g >> 1) & 3)) * 16));
+              *reinterpret_cast<const uint32_t*>(at + r * kTile + h * 8 * kRow + j * 16);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) q[h][i] = unpack<T>(word, i, magic, off);
+          for (int i = 0; i < 4; ++i) q[h][i] = unpack<T>(word, i, mask, magic, off);
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -266,7 +272,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ?
 template <typename T, int RT, int NT, int FL, bool ZP, int S>
 int launch_ring(const Int4Args& a, cudaStream_t st) {
   const int mt = a.M < 8 * NT ? a.M : 8 * NT;
-  const int ring = kWarps * S * (RT * 1024 + mt * 256), part = kWarps * mt * 16 * RT * 4;
+  const int ring = kWarps * S * (RT * kTile + mt * kTok), part = kWarps * mt * 16 * RT * 4;
   const int smem = ring > part ? ring : part;
   const auto kernel = int4_kernel<T, RT, NT, FL, ZP, S>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
