@@ -59,4 +59,11 @@ __device__ __forceinline__ float block_max_all(float v, float* red) {
   return warp_max(l < nw ? red[l] : -INFINITY);
 }
 
+// A value in another rank's shared memory (address from mapa_shared).
+__device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 }  // namespace brain

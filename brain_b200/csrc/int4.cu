@@ -2,22 +2,29 @@
 //   w[n, k] = s[n, g] (v[n, k] - z[n, g]),  g = k / G,
 // with two values v a byte (low nibble first): two's complement without zero points, 0 .. 15 with them.
 //
-// The values minus their zero point are small whole numbers, exact in 16 bits; products and sums are f32,
-// a group's sum is multiplied by its scale in f32, and y is rounded once.
+// Bound by memory: N K / 2 bytes of weights and their scales, read once for all tokens of a call. What stands
+// in the way is unpacking: at the memory's rate an SM has about 40 cycles for 1 KB of weights (2048 values), and
+// its logic pipe does 64 operations a cycle. The tensor cores' warp-level 16 x 8 x 16 product takes 16 output
+// rows of the weight as its rows and 8 tokens as its columns. Its order along K is free as long as both sides
+// agree, so a lane takes the pairs (i, i + 4) that a shift and a mask leave in the two halves of a word of eight
+// values, and pairs the activations alike.
+//   bf16: a nibble masked onto the exponent bits of 128 is 128 + v exactly, and stays so: the group's sum less
+//     (128 + offset) times the group's sum of x, which a product with ones gives once. That costs the f32 sum of
+//     128 products up to 8 roundings at 34 times the size of its terms, 8e-6 of sum |x w|, against 2^-9 of y.
+//   f16: on the exponent bits of 1024 the same would cost eight times that, near f16's own step. There the
+//     offset comes off each pair, exactly: 1024 + v less 1024 + offset for a low nibble, and for a high one,
+//     which stands for 1024 + 16 v where it is, a 16th of that less 64 + offset, with no shift.
+// (Operands of 8 bits were slower: e4m3, which holds 0 .. 15, is taken apart into 16-bit products on this chip,
+// and whole numbers need three digits of each token and their sums put together.)
 //
-// Bound by memory: N K / 2 bytes of weights and their scales, read once for all tokens of a call.
-//
-// The tensor cores' warp-level 16 x 8 x 16 product takes 16 output rows of the weight as its rows and 8
-// tokens as its columns, so one to eight tokens cost the same. Its operand order along K is free as long as
-// both sides agree: a lane takes the 8 values of one 32-bit word of its row at a time, the pairs (i, i + 4)
-// that a shift and a mask leave in the two halves of a register, and pairs the activations alike. Masked
-// onto the exponent bits of 128 (bf16) or 1024 (f16) a nibble is that number plus its value; one packed
-// subtraction takes the base and the zero point off, exactly.
-//
-// A CTA owns 16 RT output rows, its 8 warps split K in pairs of 128-wide chunks. Weights and activations of a
-// chunk come through a ring of asynchronous copies that each warp runs for itself (no block barrier in the
-// loop, as many bytes in flight as shared memory holds); the scales of a chunk are requested when its copies
-// are. The warps' sums meet in shared memory in a fixed order.
+// A warp owns 256 of K for the whole call and keeps its tokens' operand registers; it streams tiles of 32 rows
+// of its K through a ring of TMA copies of its own, with no barrier to other warps. Eight warps make a CTA, a
+// cluster of CTAs covers K, and clusters take even shares of the rows. Every second tile the warps' sums meet in
+// shared memory, and go on to the shared memory of the CTA that owns them; the cluster's barrier comes every
+// kRound of those meetings and is waited for only when the next kRound are done. All sums are added in a fixed
+// order.
+#include <type_traits>
+
 #include "elem.cuh"
 
 using namespace brain;
@@ -25,299 +32,441 @@ using namespace brain;
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kChunk = 128;  // K of one ring stage: 64 bytes of a weight row, 256 of a token
-// rows in the ring: 64 + 16 and 256 + 64 bytes put the 8 rows (tokens) that a warp reads at once on other banks
-constexpr int kRow = 80, kTile = 16 * kRow, kTok = 320;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTiles = 2;         // 32-row tiles between two meetings of the warps
+constexpr int kRound = 4;         // meetings of the warps between two of the cluster
+constexpr int kMaxCluster = 16;
 
 struct Int4Args {
   const void* x;      // [M, K]
   int64_t ldx;
-  const uint8_t* w;   // [N, K / 2]
-  int64_t ldw;
   const void* s;      // [N, groups]
   const uint8_t* z;   // [N, groups] or null
   const void* bias;   // [N] or null
+  const float* prev;  // [M, N] sums of earlier K to add, or null
+  float* next;        // [M, N] where the sums go when more K follows, or null
   void* y;            // [M, N]
-  int M, N, K, groups;
+  int M, N, K, groups, group0;  // group0: the group that this K starts in
   // k / G of a k that 32 divides is the high half of (k / 32) inv_g, inv_g the next whole number above
   // 2^32 / (G / 32): exact while (k / 32) (G / 32) < 2^32, and G <= K <= 2^20. 0: G is 32
   uint32_t inv_g;
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where !on
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+// c += A B: A 16 x 16, B 16 x 8
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+template <>
+__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename T>
-struct Half2;  // the pair type, its exponent base and the product
-template <>
-struct Half2<__nv_bfloat16> {
-  static constexpr uint32_t kBase = 0x43004300u;  // 128, 128
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-template <>
-struct Half2<__half> {
-  static constexpr uint32_t kBase = 0x64006400u;  // 1024, 1024
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-
-// Pair i of a word of 8 values: (value i, value i + 4) less the offset that `off` holds, as T. `magic` is the
-// base's exponent, with bit 3 set where the values are two's complement (which makes them an offset of 8).
-template <typename T>
-__device__ __forceinline__ uint32_t unpack(uint32_t w, int i, uint32_t mask, uint32_t magic, uint32_t off) {
+// (w & mask) ^ flip in one operation
+__device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t flip) {
   uint32_t v;
-  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(v) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));  // (w & mask) ^ magic
-  return Half2<T>::sub(v, off);
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(v) : "r"(w), "r"(mask), "r"(flip));
+  return v;
 }
+
+// The four pairs (i, i + 4) of a word: as 128 + v for bf16, less their offset for f16. Two's complement values
+// have their top bit flipped, which makes them an offset of 8. The constants are held in registers.
+template <typename T, bool ZP>
+struct Unpack;
+template <bool ZP>
+struct Unpack<__nv_bfloat16, ZP> {
+  uint32_t mask, flip;
+  __device__ __forceinline__ Unpack() {
+    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
+    asm volatile("mov.b32 %0, %1;" : "=r"(flip) : "n"(ZP ? 0x43004300 : 0x43084308));
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, int, uint32_t (&q)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = pick(w >> (4 * i), mask, flip);
+  }
+};
+template <bool ZP>
+struct Unpack<__half, ZP> {
+  uint32_t mask, flip, high_mask, high_flip;
+  __device__ __forceinline__ Unpack() {
+    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
+    asm volatile("mov.b32 %0, 0x00f000f0;" : "=r"(high_mask));
+    asm volatile("mov.b32 %0, %1;" : "=r"(flip) : "n"(ZP ? 0x64006400 : 0x64086408));
+    asm volatile("mov.b32 %0, %1;" : "=r"(high_flip) : "n"(ZP ? 0x64006400 : 0x64806480));
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, int off, uint32_t (&q)[4]) const {
+    const __half2 low = __float2half2_rn(-1024.f - off), high = __float2half2_rn(-64.f - off);
+    const __half2 sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const uint32_t l = pick(w >> (4 * i), mask, flip), h = pick(w >> (4 * i), high_mask, high_flip);
+      const __half2 a = __hadd2(*reinterpret_cast<const __half2*>(&l), low);
+      const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&h), sixteenth, high);
+      q[i] = *reinterpret_cast<const uint32_t*>(&a);
+      q[i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+};
 
 __device__ __forceinline__ uint32_t group_of(uint32_t k32, uint32_t inv_g) {
   return inv_g ? __umulhi(k32, inv_g) : k32;
 }
 
-// RT: 16-row tiles a CTA; NT: 8-token tiles; FL: scales a row and chunk (128 / G, at least 1); ZP: zero points;
-// S: ring stages.
-template <typename T, int RT, int NT, int FL, bool ZP, int S>
-__global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 1 : NT == 1 && FL < 4 ? 3 : 2) int4_kernel(Int4Args a) {
-  extern __shared__ __align__(16) uint8_t smem[];
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+// for a warp that has written nothing that another CTA reads
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// NT: 8-token tiles; KB: 32-wide K blocks a warp. A unit is 16 rows by 8 tokens.
+template <int NT, int KB>
+struct Layout {
+  static constexpr int kStages = 2;                     // tiles in a warp's ring
+  static constexpr int kTile = 32 * KB * 16;            // bytes of a tile of a warp's K
+  static constexpr int kRing = kWarps * kStages * kTile;
+  static constexpr int kUnits = kTiles * 2 * NT;
+  static constexpr int kPart = kUnits * kWarps * 512;   // [unit][warp][lane] float4
+  static constexpr int places(int split) { return (kUnits * kRound + split - 1) / split; }
+  static constexpr int recv(int split) { return split > 1 ? 2 * places(split) * split * 512 : 0; }
+  // recv is largest where split does not divide a round
+  static constexpr int kMost = 2 * (kUnits * kRound + kMaxCluster - 1) * 512;
+  static constexpr int smem(int split) { return 1024 + kRing + kPart + recv(split) + kWarps * kStages * 8 + 16; }
+};
+
+// FL: groups that a scale may change at in 128 of K (128 / G, at least 1); ZP: zero points.
+template <typename T, int NT, int KB, int FL, bool ZP>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+    int4_kernel(const __grid_constant__ CUtensorMap wmap, const Int4Args a) {
+  using L = Layout<NT, KB>;
+  constexpr int kGroups = KB / 4 * FL;  // sums taken apart in a warp's K
+  constexpr int kGroupBlocks = KB / kGroups, kStages = L::kStages, kUnits = L::kUnits;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const int split = gridDim.x, rank = blockIdx.x;
+  float4* part = reinterpret_cast<float4*>(smem + L::kRing);
+  float4* recv = reinterpret_cast<float4*>(smem + L::kRing + L::kPart);
+  uint8_t* tail = smem + L::kRing + L::kPart + L::recv(split);
+  int* abort_flag = reinterpret_cast<int*>(tail + kWarps * kStages * 8);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
-  const int n0 = blockIdx.x * 16 * RT, m0 = blockIdx.y * 8 * NT, mt = min(8 * NT, a.M - m0);
-  const uint32_t stage_bytes = RT * kTile + mt * kTok;
-  const uint8_t* ring = smem + warp * S * stage_bytes;
-  const int chunks = (a.K + kChunk - 1) / kChunk;
-  // chunk pairs (a 128-byte line of every row) go round the warps
-  const int whole = chunks / (2 * kWarps), rest = min(max(chunks - whole * 2 * kWarps - 2 * warp, 0), 2);
-  const int mine = 2 * whole + rest;
-  // in registers, so that one three-input operation masks a pair and sets its exponent
-  uint32_t mask, magic;
-  asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
-  asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(ZP ? Half2<T>::kBase : Half2<T>::kBase ^ 0x00080008u));
+  const uint32_t bars = smem_u32(tail) + warp * kStages * 8, ring = smem_u32(smem) + warp * kStages * L::kTile;
 
-  // one base for the CTA, 32-bit offsets for its lanes; rows past the end repeat the last, and are not stored
-  const uint8_t* wbase = a.w + n0 * a.ldw;
-  const T* sbase = (const T*)a.s + (int64_t)n0 * a.groups;
-  const uint8_t* zbase = ZP ? a.z + (int64_t)n0 * a.groups : nullptr;
-  const uint8_t* xbase = (const uint8_t*)a.x + m0 * a.ldx * 2;
-  uint32_t woff[RT][2], soff[RT][2];
+  const int tiles = (a.N + 31) / 32, m0 = blockIdx.z * 8 * NT;
+  const int t0 = (int)((int64_t)tiles * blockIdx.y / gridDim.y), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / gridDim.y);
+  const int k0 = (rank * kWarps + warp) * KB * 32;
+  const bool active = k0 < a.K;
+
+  if (threadIdx.x == 0) *abort_flag = 0;
+  const auto fetch = [&](int t, int st) {
+    mbar_arrive_expect_tx(bars + 8 * st, L::kTile);
+    tma_load_2d(&wmap, ring + st * L::kTile, bars + 8 * st, k0 / 2, t * 32);
+  };
+  if (lane == 0) {
+    for (int st = 0; st < kStages; ++st) mbar_init(bars + 8 * st, 1);
+    fence_barrier_init();
+    if (active)
+      for (int st = 0; st < kStages && t0 + st < t1; ++st) fetch(t0 + st, st);
+  }
+  __syncthreads();
+  if (split > 1) cluster_arrive_relaxed();
+
+  // ---- this warp's tokens: the pairs of token t * 8 + g, and (bf16) the groups' sums of tokens t4 * 2, + 1
+  constexpr bool kSums = std::is_same<T, __nv_bfloat16>::value;
+  uint32_t b[NT][KB][4];
+  float xsum[NT][kGroups][2];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+  for (int t = 0; t < NT; ++t) {
+    const int m = m0 + t * 8 + g;
+    const uint8_t* row = (const uint8_t*)a.x + (m * a.ldx + k0 + t4 * 8) * 2;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t n = min(r * 16 + h * 8 + g, a.N - 1 - n0);
-      woff[r][h] = n * (uint32_t)a.ldw;
-      soff[r][h] = n * a.groups;
+    for (int j = 0; j < KB; ++j) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (m < a.M && k0 + j * 32 < a.K) v = *reinterpret_cast<const uint4*>(row + j * 64);
+      b[t][j][0] = __byte_perm(v.x, v.z, 0x5410);
+      b[t][j][1] = __byte_perm(v.x, v.z, 0x7632);
+      b[t][j][2] = __byte_perm(v.y, v.w, 0x5410);
+      b[t][j][3] = __byte_perm(v.y, v.w, 0x7632);
     }
-  const uint32_t wdst = smem_u32(ring) + g * kRow + t4 * 16;
-  const uint32_t xdst = smem_u32(ring) + RT * kTile + (lane / 16) * kTok + (lane & 15) * 16;
-  const uint32_t xoff = (lane / 16) * (uint32_t)a.ldx * 2;
+    if (kSums)
+#pragma unroll
+      for (int q = 0; q < kGroups; ++q) {
+        const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        float c[4] = {};
+#pragma unroll
+        for (int j = q * kGroupBlocks; j < (q + 1) * kGroupBlocks; ++j) {
+          mma<T>(c, ones, b[t][j][0], b[t][j][1]);
+          mma<T>(c, ones, b[t][j][2], b[t][j][3]);
+        }
+        xsum[t][q][0] = c[0];
+        xsum[t][q][1] = c[1];
+      }
+  }
 
-  auto first_k = [&](int it) { return (((it >> 1) * kWarps + warp) * 2 + (it & 1)) * kChunk; };
-  auto fetch = [&](int it, int st) {
-    if (it < mine) {
-      const int k0 = first_k(it);
-      const uint32_t stage = st * stage_bytes;
-      const bool on = k0 + t4 * 32 < a.K;
-      const uint32_t kw = on ? k0 / 2 + t4 * 16 : 0;
+  // ---- scales and zero points of a tile's rows g, g + 8, .., asked for when the last tile is done
+  T sc[4][kGroups];
+  uint8_t zp[4][kGroups];
+  uint32_t goff[kGroups];
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+  for (int q = 0; q < kGroups; ++q)
+    goff[q] = min(a.group0 + (int)group_of(k0 / 32 + q * kGroupBlocks, a.inv_g), a.groups - 1);
+  const auto scales = [&](int t) {
+    const int64_t first = (int64_t)t * 32 * a.groups;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) copy16(wdst + stage + r * kTile + h * 8 * kRow, wbase + (woff[r][h] + kw), on);
-      const bool xon = k0 + (g & 3) * 32 < a.K;
-      const uint32_t kx = xon ? xoff + (k0 + (lane & 15) * 8) * 2 : 0;
+    for (int h = 0; h < 4; ++h) {
+      const uint32_t row = min(h * 8 + g, a.N - 1 - t * 32) * a.groups;  // rows past the end are not stored
 #pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) {
-        const int tok = lane / 16 + 2 * i;
-        if (tok < mt)
-          copy16(xdst + stage + i * 2 * kTok, xbase + (kx + (xon ? i * (uint32_t)a.ldx * 4 : 0)), xon);
+      for (int q = 0; q < kGroups; ++q) {
+        sc[h][q] = ((const T*)a.s + first)[row + goff[q]];
+        if (ZP) zp[h][q] = (a.z + first)[row + goff[q]];
       }
     }
-    copy_commit();
   };
-  // the scales (and zero points) of a chunk, asked for one chunk ahead
-  T sc[RT][2][FL], scn[RT][2][FL];
-  uint8_t zp[RT][2][FL], zpn[RT][2][FL];
-  auto scales = [&](int it) {
-    if (it < mine) {
-      const uint32_t k32 = first_k(it) / 32;
+  if (active && t0 < t1) scales(t0);
+
+  // unit u of a round belongs to rank u % split, in place u / split
+  const int places = L::places(split);
+  const auto store = [&](int t, int u, float4 v) {  // unit u of the tile t: row half u / NT, tokens u % NT
+    const int n = t * 32 + u / NT * 16 + g, m = m0 + (u % NT) * 8 + t4 * 2;
+    const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int f = 0; f < FL; ++f) {
-        const uint32_t grp = min((int)group_of(k32 + f * (4 / FL), a.inv_g), a.groups - 1);
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            scn[r][h][f] = sbase[soff[r][h] + grp];
-            if (ZP) zpn[r][h][f] = zbase[soff[r][h] + grp];
-          }
+    for (int c = 0; c < 4; ++c) {
+      const int nn = n + (c / 2) * 8, mm = m + (c & 1);
+      if (nn >= a.N || mm >= a.M) continue;
+      const int64_t at = (int64_t)mm * a.N + nn;
+      float r = f[c] + (a.prev ? a.prev[at] : 0.f);
+      if (a.next) {
+        a.next[at] = r;
+      } else {
+        if (a.bias) r += to_f32(((const T*)a.bias)[nn]);
+        ((T*)a.y)[at] = from_f32<T>(r);
       }
     }
   };
+  const auto finish = [&](int tr, int parity) {  // the owned units of the round that starts at tile tr
+    for (int i = warp; i < places; i += kWarps) {
+      const int u = i * split + rank, t = tr + u / (2 * NT);
+      if (u >= kUnits * kRound || t >= t1) continue;
+      const float4* from = recv + ((parity * places + i) * split) * 32 + lane;
+      float4 v = from[0];
+      for (int r = 1; r < split; ++r) {
+        const float4 w = from[r * 32];
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
+      store(t, u % (2 * NT), v);
+    }
+  };
 
-  float sum[RT][NT][4] = {};
-#pragma unroll
-  for (int st = 0; st < S - 1; ++st) fetch(st, st);
-  scales(0);
-  int st = 0;
+  const Unpack<T, ZP> unpack;
+  const uint8_t* wlane = smem + warp * kStages * L::kTile + g * (KB * 16) + t4 * 4;
+  const uint32_t turn = (KB == 8 ? g : (g >> 1) & 3) * 16;  // the copy's swizzle of 16-byte blocks
+  int st = 0, parity = 0, meeting = 0;  // meeting: of the round
+  uint32_t phase = 0;
+  for (int tb = t0; tb < t1; tb += kTiles) {
+    const bool closes = meeting == kRound - 1 || tb + kTiles >= t1;
+    if (tb > t0) asm volatile("bar.sync 1, 512;" ::: "memory");  // the last meeting's sums have been read
 #pragma unroll 1
-  for (int it = 0; it < mine; ++it) {
-    copy_wait<S - 2>();
-    __syncwarp();
-    fetch(it + S - 1, st == 0 ? S - 1 : st - 1);
+    for (int i = 0; i < kTiles; ++i) {
+      const int t = tb + i;
+      float sum[2][NT][4] = {};
+      if (active && t < t1) {
+        mbar_wait(bars + 8 * st, phase, BRAIN_ERR_TIMEOUT_FULL, 801, abort_flag);
+        const uint8_t* at = wlane + st * L::kTile;
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+        for (int q = 0; q < kGroups; ++q) {
+          float acc[2][NT][4] = {};
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+          for (int j = q * kGroupBlocks; j < (q + 1) * kGroupBlocks; ++j) {
+            const uint8_t* aj = at + (turn ^ (j * 16));
 #pragma unroll
-        for (int f = 0; f < FL; ++f) {
-          sc[r][h][f] = scn[r][h][f];
-          if (ZP) zp[r][h][f] = zpn[r][h][f];
-        }
-    scales(it + 1);
-    const uint8_t* at = ring + st * stage_bytes + g * kRow + t4 * 4;
-    const uint8_t* xs = ring + st * stage_bytes + RT * kTile + t4 * 16;
-    st = st == S - 1 ? 0 : st + 1;
-    float acc[RT][NT][4] = {};
+            for (int r = 0; r < 2; ++r) {
+              uint32_t w[2][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t b[NT][4];
+              for (int h = 0; h < 2; ++h)
+                unpack(*reinterpret_cast<const uint32_t*>(aj + (r * 2 + h) * 8 * (KB * 16)), ZP ? zp[r * 2 + h][q] : 8, w[h]);
+              const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int tok = min(t * 8 + g, mt - 1);  // columns past the last token are not stored
-        const uint4 v = *reinterpret_cast<const uint4*>(xs + tok * kTok + j * 64);
-        b[t][0] = __byte_perm(v.x, v.z, 0x5410);
-        b[t][1] = __byte_perm(v.x, v.z, 0x7632);
-        b[t][2] = __byte_perm(v.y, v.w, 0x5410);
-        b[t][3] = __byte_perm(v.y, v.w, 0x7632);
-      }
+              for (int n = 0; n < NT; ++n) {
+                mma<T>(acc[r][n], a0, b[n][j][0], b[n][j][1]);
+                mma<T>(acc[r][n], a1, b[n][j][2], b[n][j][3]);
+              }
+            }
+          }
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        uint32_t q[2][4];
+          for (int h = 0; h < 4; ++h) {
+            const float s = to_f32(sc[h][q]);
+            const float off = ZP ? __int_as_float(0xcb000000u | zp[h][q]) + (8388608.f - 128.f) : -136.f;  // -128 - z
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t off = ZP ? Half2<T>::kBase + zp[r][h][j * FL / 4] * 0x00010001u : magic;
-          const uint32_t word =
-              *reinterpret_cast<const uint32_t*>(at + r * kTile + h * 8 * kRow + j * 16);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) q[h][i] = unpack<T>(word, i, mask, magic, off);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          Half2<T>::mma(acc[r][t], q[0][0], q[1][0], q[0][1], q[1][1], b[t][0], b[t][1]);
-          Half2<T>::mma(acc[r][t], q[0][2], q[1][2], q[0][3], q[1][3], b[t][2], b[t][3]);
-        }
-        if ((j + 1) % (4 / FL) == 0) {  // the end of a group, or of the chunk in a wider one
-          const float s0 = to_f32(sc[r][0][j * FL / 4]), s1 = to_f32(sc[r][1][j * FL / 4]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            sum[r][t][0] = fmaf(s0, acc[r][t][0], sum[r][t][0]);
-            sum[r][t][1] = fmaf(s0, acc[r][t][1], sum[r][t][1]);
-            sum[r][t][2] = fmaf(s1, acc[r][t][2], sum[r][t][2]);
-            sum[r][t][3] = fmaf(s1, acc[r][t][3], sum[r][t][3]);
-            acc[r][t][0] = acc[r][t][1] = acc[r][t][2] = acc[r][t][3] = 0.f;
+              for (int c = 0; c < 2; ++c) {
+                float& to = sum[h / 2][n][h % 2 * 2 + c];
+                const float v = acc[h / 2][n][h % 2 * 2 + c];
+                to = fmaf(s, kSums ? fmaf(off, xsum[n][q][c], v) : v, to);
+              }
           }
         }
+        __syncwarp();
+        if (lane == 0 && t + kStages < t1) fetch(t + kStages, st);
+        if (t + 1 < t1) scales(t + 1);
+        st = st == kStages - 1 ? 0 : st + 1;
+        phase ^= st == 0;
       }
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          part[(((i * 2 + r) * NT + n) * kWarps + warp) * 32 + lane] =
+              make_float4(sum[r][n][0], sum[r][n][1], sum[r][n][2], sum[r][n][3]);
+    }
+    __syncthreads();
+    if (split > 1 && meeting == 0) {
+      cluster_wait();  // at first: every CTA of the cluster runs; later: the last round's sums are here
+      if (tb > t0) finish(tb - kTiles * kRound, parity ^ 1);
+      __syncwarp();
+    }
+    for (int u = warp; u < kUnits; u += kWarps) {
+      if (tb + u / (2 * NT) >= t1) continue;
+      const float4* from = part + u * kWarps * 32 + lane;
+      float4 v = from[0];
+#pragma unroll
+      for (int k = 1; k < kWarps; ++k) {
+        const float4 w = from[k * 32];
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
+      if (split > 1) {
+        const int ur = meeting * kUnits + u;
+        const uint32_t to =
+            mapa_shared(smem_u32(recv + ((parity * places + ur / split) * split + rank) * 32 + lane), ur % split);
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                     : "memory");
+      } else {
+        store(tb + u / (2 * NT), u % (2 * NT), v);
+      }
+    }
+    __syncwarp();
+    if (tb + kTiles < t1) asm volatile("bar.arrive 1, 512;" ::: "memory");
+    if (closes) {
+      if (split > 1) {
+        if (warp < kUnits)
+          cluster_arrive();
+        else
+          cluster_arrive_relaxed();
+      }
+      meeting = 0;
+      parity ^= 1;
+    } else {
+      ++meeting;
     }
   }
-  copy_wait<0>();
-  __syncthreads();
-  // [warp][token][row] partial sums over the ring's place
-  constexpr int kRows = 16 * RT;
-  float* part = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int tok = t * 8 + t4 * 2 + (c & 1), row = r * 16 + (c / 2) * 8 + g;
-        if (tok < mt) part[(warp * mt + tok) * kRows + row] = sum[r][t][c];
-      }
-  __syncthreads();
-  for (int i = threadIdx.x; i < mt * kRows; i += kWarps * 32) {
-    const int n = n0 + i % kRows;
-    if (n >= a.N) continue;
-    float v = 0.f;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) v += part[k * mt * kRows + i];
-    if (a.bias) v += to_f32(((const T*)a.bias)[n]);
-    ((T*)a.y)[(int64_t)(m0 + i / kRows) * a.N + n] = from_f32<T>(v);
+  if (split > 1) {
+    cluster_wait();
+    if (t1 > t0) finish(t0 + (t1 - t0 - 1) / (kTiles * kRound) * (kTiles * kRound), parity ^ 1);
   }
 }
 
-template <typename T, int RT, int NT, int FL, bool ZP, int S>
-int launch_ring(const Int4Args& a, cudaStream_t st) {
-  const int mt = a.M < 8 * NT ? a.M : 8 * NT;
-  const int ring = kWarps * S * (RT * kTile + mt * kTok), part = kWarps * mt * 16 * RT * 4;
-  const int smem = ring > part ? ring : part;
-  const auto kernel = int4_kernel<T, RT, NT, FL, ZP, S>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <typename T, int NT, int KB, int FL, bool ZP>
+int launch_tile(const Int4Args& a, const uint8_t* w, int64_t ldw, cudaStream_t st) {
+  using L = Layout<NT, KB>;
+  CUtensorMap wmap;
+  const uint64_t wd[2] = {(uint64_t)a.K / 2, (uint64_t)a.N}, ws[1] = {(uint64_t)ldw};
+  const uint32_t wb[2] = {KB * 16, 32};
+  if (!brain_host::encode_tiled(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(w), wd, ws, wb,
+                                KB == 8 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+    return (int)cudaErrorInvalidValue;
+  const auto kernel = int4_kernel<T, NT, KB, FL, ZP>;
+  const int per = kWarps * KB * 32, split = (a.K + per - 1) / per, tiles = (a.N + 31) / 32;
+  const int ntok = (a.M + 8 * NT - 1) / (8 * NT);
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = L::smem(split);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = split;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  // clusters of this size that the device runs at once, by device
+  static int resident[64][kMaxCluster + 1] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  const dim3 grid((a.N + 16 * RT - 1) / (16 * RT), (a.M + 8 * NT - 1) / (8 * NT));
-  kernel<<<grid, kWarps * 32, smem, st>>>(a);
-  return (int)cudaGetLastError();
+  int& fit = resident[dev & 63][split];
+  if (fit == 0) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(1) + L::kMost);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cfg.gridDim = dim3(split, 1, 1);
+    int n = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess) return (int)e;
+    if (n <= 0) return (int)cudaErrorInvalidConfiguration;
+    fit = n;
+  }
+  const int share = fit / ntok > 1 ? fit / ntok : 1;
+  cfg.gridDim = dim3(split, tiles < share ? tiles : share, ntok);
+  return (int)cudaLaunchKernelEx(&cfg, kernel, wmap, a);
 }
 
 template <typename T, int FL, bool ZP>
-int launch_tokens(const Int4Args& a, cudaStream_t st) {
-  if (a.M <= 8) return launch_ring<T, 2, 1, FL, ZP, 3>(a, st);
-  if (a.M <= 16) return launch_ring<T, 2, 2, FL, ZP, 2>(a, st);
-  return launch_ring<T, 2, 4, FL, ZP, 2>(a, st);
+int launch_tokens(const Int4Args& a, const uint8_t* w, int64_t ldw, cudaStream_t st) {
+  if (a.M <= 8) return launch_tile<T, 1, 8, FL, ZP>(a, w, ldw, st);
+  return launch_tile<T, 2, 8, FL, ZP>(a, w, ldw, st);
 }
 
 template <typename T, bool ZP>
-int launch_groups(const Int4Args& a, int G, cudaStream_t st) {
-  // a scale may change inside a chunk: every 64 values, or at any multiple of 32
-  if (G % kChunk == 0) return launch_tokens<T, 1, ZP>(a, st);
-  if (G % 64 == 0) return launch_tokens<T, 2, ZP>(a, st);
-  return launch_tokens<T, 4, ZP>(a, st);
+int launch_groups(const Int4Args& a, int G, const uint8_t* w, int64_t ldw, cudaStream_t st) {
+  // a scale may change inside 128 of K: every 64 values, or at any multiple of 32
+  if (G % 128 == 0) return launch_tokens<T, 1, ZP>(a, w, ldw, st);
+  if (G % 64 == 0) return launch_tokens<T, 2, ZP>(a, w, ldw, st);
+  return launch_tokens<T, 4, ZP>(a, w, ldw, st);
 }
 
 template <typename T>
-int launch(const Int4Args& a, int G, cudaStream_t st) {
-  return a.z ? launch_groups<T, true>(a, G, st) : launch_groups<T, false>(a, G, st);
+int launch(Int4Args a, int G, const uint8_t* w, int64_t ldw, float* sums, cudaStream_t st) {
+  // a cluster covers kMaxCluster x 2048 of K; longer rows go slab by slab, their sums through `sums`
+  constexpr int kSlab = kMaxCluster * 2048;
+  const int K = a.K;
+  const T* x = (const T*)a.x;
+  if (K > kSlab && (!sums || kSlab % G)) return (int)cudaErrorInvalidValue;
+  for (int k = 0; k < K; k += kSlab) {
+    a.x = x + k;
+    a.K = K - k < kSlab ? K - k : kSlab;
+    a.group0 = k / G;
+    a.prev = k ? sums : nullptr;
+    a.next = k + kSlab < K ? sums : nullptr;
+    const int e = a.z ? launch_groups<T, true>(a, G, w + k / 2, ldw, st) : launch_groups<T, false>(a, G, w + k / 2, ldw, st);
+    if (e) return e;
+  }
+  return 0;
 }
 
 }  // namespace
 
-// K and G multiples of 32, groups = ceil(K / G); w and x rows 16-byte aligned; y [M, N] contiguous.
+BRAIN_STATUS_READER(int4)
+
+// K and G multiples of 32, groups = ceil(K / G); w and x rows 16-byte aligned; y [M, N] contiguous; sums [M, N]
+// f32 where K > 32768 (which G then has to divide), else unused.
 BRAIN_API int brain_int4_linear(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* s,
-                                const void* z, const void* bias, void* y, int M, int N, int K, int G,
+                                const void* z, const void* bias, void* y, float* sums, int M, int N, int K, int G,
                                 cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0 || K % 32 || G <= 0 || G % 32 || ldw % 16 || ((uintptr_t)w & 15) || ldx % 8 || ((uintptr_t)x & 15) ||
-      M > 8 * 65535 || K > (1 << 20) || ldw > (1 << 26) || ldx > (1 << 26))
+      M > 8 * 65535 || K > (1 << 20))
     return (int)cudaErrorInvalidValue;
+  const int groups = (K + G - 1) / G;
   if (G > K) G = K;
   const uint32_t inv_g = G == 32 ? 0 : (uint32_t)((1ull << 32) / (G / 32)) + 1;
-  const Int4Args a{x, ldx, (const uint8_t*)w, ldw, s, (const uint8_t*)z, bias, y, M, N, K, (K + G - 1) / G, inv_g};
+  const Int4Args a{x, ldx, s, (const uint8_t*)z, bias, nullptr, nullptr, y, M, N, K, groups, 0, inv_g};
   switch (dtype) {
-    case BRAIN_BF16: return launch<__nv_bfloat16>(a, G, st);
-    case BRAIN_F16: return launch<__half>(a, G, st);
+    case BRAIN_BF16: return launch<__nv_bfloat16>(a, G, (const uint8_t*)w, ldw, sums, st);
+    case BRAIN_F16: return launch<__half>(a, G, (const uint8_t*)w, ldw, sums, st);
   }
   return (int)cudaErrorInvalidValue;
 }

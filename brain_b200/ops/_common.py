@@ -54,11 +54,12 @@ _native.register({
     "brain_distill_reduce": ("brain_kernels", "plppps"),
     "brain_status_distill": ("brain_kernels", "pi"),
     "brain_verify_draft": ("brain_kernels", "ipllpllpppppliis"),
-    "brain_int4_linear": ("brain_kernels", "iplplppppiiiis"),
+    "brain_status_int4": ("brain_kernels", "pi"),
+    "brain_int4_linear": ("brain_kernels", "iplplpppppiiiis"),
 })
 
 STATUS_TAGS = ["gemm", "norms", "elementwise", "ce", "optim", "attention", "attention_tc", "attention_bwd_tc",
-               "attention_decode", "decode_tp", "distill"]
+               "attention_decode", "decode_tp", "distill", "int4"]
 
 
 def same_device(ref: torch.Tensor, *others) -> None:

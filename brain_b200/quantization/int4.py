@@ -15,11 +15,16 @@ import torch
 from ..ops._common import dtype_code, launch, no_backward, ptr, rows2d, same_device
 
 
+_SLAB = 32768  # inputs that one launch covers: longer rows go in several, their sums kept in float32
+
+
 def _check_group(K: int, group_size: int) -> None:
     if group_size <= 0 or group_size % 32:
         raise ValueError(f"group size {group_size} is not a positive multiple of 32")
-    if K <= 0 or K % 32:
-        raise ValueError(f"{K} input features: a multiple of 32 is needed")
+    if K <= 0 or K % 32 or K > 2 ** 20:
+        raise ValueError(f"{K} input features: a multiple of 32 up to 2^20 is needed")
+    if K > _SLAB and _SLAB % group_size:
+        raise ValueError(f"group size {group_size} does not divide {_SLAB}, as more inputs than that need it to")
 
 
 def quantize_int4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True,
@@ -97,9 +102,10 @@ def int4_linear(x, packed, scales, zeros=None, bias=None, group_size: int = 128)
     if x2.stride(0) % 8 or x2.data_ptr() % 16:  # the kernel copies 16 bytes at a time
         x2 = x2.clone(memory_format=torch.contiguous_format)
     y = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
+    sums = torch.empty(x2.shape[0], N, device=x.device, dtype=torch.float32) if K > _SLAB else None
     launch(x, "brain_int4_linear", code, x2.data_ptr(), x2.stride(0), packed.data_ptr(), packed.stride(0),
            scales.contiguous().data_ptr(), None if zeros is None else zeros.contiguous().data_ptr(), ptr(bias),
-           y.data_ptr(), x2.shape[0], N, K, group_size)
+           y.data_ptr(), ptr(sums), x2.shape[0], N, K, group_size)
     return y
 
 

@@ -76,6 +76,7 @@ def test_refusals():
                 lambda: Q.int4_linear(x, packed, scales, z, torch.zeros(7).bfloat16(), 64),
                 lambda: Q.int4_linear(x, packed.int(), scales, z, group_size=64),
                 lambda: Q.quantize_int4(torch.zeros(4, 48), 32),
+                lambda: Q.quantize_int4(torch.zeros(1, 96 * 384), 96),
                 lambda: Q.quantize_int4(torch.zeros(64), 32)):
         with pytest.raises(ValueError):
             bad()
@@ -96,7 +97,8 @@ def test_refusals():
 @pytest.mark.parametrize("M,N,K,G", [
     (1, 1, 32, 32), (1, 17, 96, 64), (2, 128, 128, 128), (8, 64, 4096, 128), (3, 100, 1376, 128), (5, 33, 4128, 32),
     (9, 48, 256, 64), (16, 250, 1024, 32), (17, 40, 2048, 96), (31, 70, 160, 4096), (33, 513, 512, 128), (64, 31, 384, 256),
-    (130, 65, 640, 64), (1, 4096, 4096, 128), (4, 1024, 14336, 128), (8, 2049, 8192, 64), (1, 3, 28672, 32)])
+    (130, 65, 640, 64), (1, 4096, 4096, 128), (4, 1024, 14336, 128), (8, 2049, 8192, 64), (1, 3, 28672, 32),
+    (3, 20, 40960, 128)])
 def test_kernel(dtype, zeros, M, N, K, G):
     packed, scales, z = weight(N, K, G, zeros, dtype, M + N)
     x = torch.randn(M, K, generator=torch.Generator().manual_seed(2)).to(dtype)
