@@ -25,7 +25,7 @@ def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_l
         raise ValueError("verify_draft takes target_probs [B, K + 1, V] and draft_tokens [B, K]")
     B, K1, V = target_probs.shape
     K = K1 - 1
-    if V == 0 or K < 0 or draft_tokens.shape != (B, K) or uniforms.shape != (B, K1):
+    if V == 0 or K < 0 or B > 65535 or draft_tokens.shape != (B, K) or uniforms.shape != (B, K1):
         raise ValueError(f"verify_draft: target_probs {tuple(target_probs.shape)}, draft_tokens "
                          f"{tuple(draft_tokens.shape)}, uniforms {tuple(uniforms.shape)}")
     if draft_probs is not None and draft_probs.shape != (B, K, V):
