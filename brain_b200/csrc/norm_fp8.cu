@@ -6,7 +6,8 @@
 // y itself is never rounded to 16 bits: the only roundings are s (what a separate addition would store)
 // and q. The floor of the scale keeps its reciprocal finite for rows of subnormal size.
 //
-// Bound by memory: 7 bytes an element at 16 bits (x, r in; s, q out) against about 12 operations.
+// Bound by memory: 7 bytes an element at 16 bits (x, r in; s, q out) against about 12 operations. A row stays in
+// registers, packed, between its two reductions, so it is read once; many rows are in flight on an SM.
 #include "elem.cuh"
 
 using namespace brain;
@@ -77,12 +78,120 @@ __global__ void __launch_bounds__(256) norm_fp8_any_kernel(const T* __restrict__
     }
 }
 
+__device__ __forceinline__ uint32_t four_e4m3(float a, float b, float c, float d) {
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (uint32_t)hi << 16;
+}
+
+// Rows of whole, aligned 16-byte vectors, VPT of them a thread. WARP: a warp a row, eight rows a CTA, no block
+// barrier (up to 128 vectors a row); else a CTA a row.
+template <typename T, int VPT, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) norm_fp8_kernel(const T* __restrict__ x, int64_t ldx,
+                                                                     const T* __restrict__ res, int64_t ldres,
+                                                                     const T* __restrict__ w, T* __restrict__ sum_out,
+                                                                     uint8_t* __restrict__ q, float* __restrict__ scales,
+                                                                     int64_t M, int D, int block, float eps) {
+  using V = Vec16<T>;
+  constexpr int N = V::N;
+  __shared__ float red[32];
+  const int64_t row = WARP ? (int64_t)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
+  const int me = WARP ? threadIdx.x % 32 : threadIdx.x, step = WARP ? 32 : blockDim.x, nvec = D / N;
+  if (WARP && row >= M) return;
+  V v[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+    if (me + i * step < nvec) v[i] = *reinterpret_cast<const V*>(x + row * ldx + (me + i * step) * N);
+  float ss = 0.f;
+  if (res) {
+    V r[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (me + i * step < nvec) r[i] = *reinterpret_cast<const V*>(res + row * ldres + (me + i * step) * N);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (me + i * step < nvec) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[i].v[e] = from_f32<T>(to_f32(v[i].v[e]) + to_f32(r[i].v[e]));
+        *reinterpret_cast<V*>(sum_out + row * D + (me + i * step) * N) = v[i];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+    if (me + i * step < nvec)
+#pragma unroll
+      for (int e = 0; e < N; ++e) ss = fmaf(to_f32(v[i].v[e]), to_f32(v[i].v[e]), ss);
+  const float rstd = rsqrtf((WARP ? warp_sum(ss) : block_sum_all(ss, red)) / D + eps);
+  // y is made twice, for the maximum and for q: holding it would take N registers a vector instead of 4
+  float amax[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    amax[i] = 0.f;
+    if (me + i * step < nvec) {
+      const V wv = *reinterpret_cast<const V*>(w + (me + i * step) * N);
+#pragma unroll
+      for (int e = 0; e < N; ++e) amax[i] = fmaxf(amax[i], fabsf(to_f32(v[i].v[e]) * rstd * to_f32(wv.v[e])));
+    }
+  }
+  float inv = 0.f;
+  if (block) {  // the 128 / N lanes with a block's vectors are neighbours
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int o = 64 / N; o > 0; o >>= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
+  } else {
+    float m = amax[0];
+#pragma unroll
+    for (int i = 1; i < VPT; ++i) m = fmaxf(m, amax[i]);
+    const float sc = scale_of(WARP ? warp_max(m) : block_max_all(m, red));
+    if (me == 0) scales[row] = sc;
+    inv = 1.f / sc;
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+    if (me + i * step < nvec) {
+      const int c = (me + i * step) * N;
+      if (block) {
+        const float sc = scale_of(amax[i]);
+        if (c % 128 == 0) scales[row * (D / 128) + c / 128] = sc;
+        inv = 1.f / sc;
+      }
+      const V wv = *reinterpret_cast<const V*>(w + c);
+      float y[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[e] = to_f32(v[i].v[e]) * rstd * to_f32(wv.v[e]) * inv;
+      if (N == 8)
+        *reinterpret_cast<uint2*>(q + row * D + c) =
+            make_uint2(four_e4m3(y[0], y[1], y[2], y[3]), four_e4m3(y[N - 4], y[N - 3], y[N - 2], y[N - 1]));
+      else
+        *reinterpret_cast<uint32_t*>(q + row * D + c) = four_e4m3(y[0], y[1], y[2], y[3]);
+    }
+}
+
 template <typename T>
 int launch(const void* x, int64_t ldx, const void* res, int64_t ldres, const void* w, void* sum, void* q, float* scales,
            int64_t M, int D, int block, float eps, cudaStream_t st) {
-  norm_fp8_any_kernel<T><<<(unsigned)M, 256, 0, st>>>((const T*)x, ldx, (const T*)res, ldres, (const T*)w, (T*)sum,
-                                                      (uint8_t*)q, scales, D, block, eps);
-  return (int)cudaGetLastError();
+  constexpr int N = 16 / sizeof(T);
+  const bool vec = D % N == 0 && ldx % N == 0 && ldres % N == 0 &&
+                   (((uintptr_t)x | (uintptr_t)res | (uintptr_t)w | (uintptr_t)sum) & 15) == 0 && ((uintptr_t)q & 7) == 0;
+  const int nvec = D / N;
+  const auto run = [&](auto kernel, int rows, int threads) {
+    kernel<<<(unsigned)((M + rows - 1) / rows), threads, 0, st>>>((const T*)x, ldx, (const T*)res, ldres, (const T*)w,
+                                                                  (T*)sum, (uint8_t*)q, scales, M, D, block, eps);
+    return (int)cudaGetLastError();
+  };
+  const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
+  if (!vec || nvec > 8192) {
+    norm_fp8_any_kernel<T><<<(unsigned)M, 256, 0, st>>>((const T*)x, ldx, (const T*)res, ldres, (const T*)w, (T*)sum,
+                                                        (uint8_t*)q, scales, D, block, eps);
+    return (int)cudaGetLastError();
+  }
+  if (nvec <= 32) return run(norm_fp8_kernel<T, 1, true>, 8, 256);
+  if (nvec <= 64) return run(norm_fp8_kernel<T, 2, true>, 8, 256);
+  if (nvec <= 128) return run(norm_fp8_kernel<T, 4, true>, 8, 256);
+  if (nvec <= 512) return run(norm_fp8_kernel<T, 2, false>, 1, threads(2));
+  if (nvec <= 1024) return run(norm_fp8_kernel<T, 4, false>, 1, threads(4));
+  return run(norm_fp8_kernel<T, 8, false>, 1, threads(8));
 }
 
 }  // namespace
