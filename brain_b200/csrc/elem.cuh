@@ -35,6 +35,41 @@ struct alignas(16) Vec16 {
   T v[N];
 };
 
+// 16 bytes as four 32-bit words, and the values of a word: two of 16 bits, or one f32.
+template <typename T>
+struct Words {
+  static constexpr int PER = 4 / sizeof(T), N = 4 * PER;
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) { f[0] = __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t pack(const float* f) { return __float_as_uint(f[0]); }
+};
+template <>
+struct Words<__nv_bfloat16> {
+  static constexpr int PER = 2, N = 8;
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+    f[0] = __uint_as_float(w << 16);
+    f[1] = __uint_as_float(w & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint32_t pack(const float* f) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f[0], f[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Words<__half> {
+  static constexpr int PER = 2, N = 8;
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    f[0] = v.x;
+    f[1] = v.y;
+  }
+  static __device__ __forceinline__ uint32_t pack(const float* f) {
+    const __half2 h = __floats2half2_rn(f[0], f[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ void set_word(uint4& v, int i, uint32_t w) { (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w) = w; }
+
 // Sum over a block of up to 32 warps; every thread gets it. `red` holds 32 values and may be reused at once.
 template <typename A>
 __device__ __forceinline__ A block_sum_all(A v, A* red) {

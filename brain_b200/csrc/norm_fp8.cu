@@ -7,7 +7,9 @@
 // and q. The floor of the scale keeps its reciprocal finite for rows of subnormal size.
 //
 // Bound by memory: 7 bytes an element at 16 bits (x, r in; s, q out) against about 12 operations. A row stays in
-// registers, packed, between its two reductions, so it is read once; many rows are in flight on an SM.
+// registers between its two reductions, so it is read once. The first kernel for this took 37 instructions an
+// element and kept the issue slots 77 % busy; so values are converted in pairs, s w is held in f32 after the
+// sum of squares, and rstd enters once a row, in the maximum and in the factor rstd / scale.
 #include "elem.cuh"
 
 using namespace brain;
@@ -87,53 +89,69 @@ __device__ __forceinline__ uint32_t four_e4m3(float a, float b, float c, float d
 // Rows of whole, aligned 16-byte vectors, VPT of them a thread. WARP: a warp a row, eight rows a CTA, no block
 // barrier (up to 128 vectors a row); else a CTA a row.
 template <typename T, int VPT, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) norm_fp8_kernel(const T* __restrict__ x, int64_t ldx,
-                                                                     const T* __restrict__ res, int64_t ldres,
-                                                                     const T* __restrict__ w, T* __restrict__ sum_out,
-                                                                     uint8_t* __restrict__ q, float* __restrict__ scales,
-                                                                     int64_t M, int D, int block, float eps) {
-  using V = Vec16<T>;
-  constexpr int N = V::N;
+__global__ void __launch_bounds__(WARP ? 256 : VPT == 4 ? 1024 : 512)
+    norm_fp8_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ res, int64_t ldres,
+                    const T* __restrict__ w, T* __restrict__ sum_out, uint8_t* __restrict__ q, float* __restrict__ scales,
+                    int64_t M, int D, int block, float eps) {
+  using W = Words<T>;
+  constexpr int N = W::N;
   __shared__ float red[32];
   const int64_t row = WARP ? (int64_t)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
   const int me = WARP ? threadIdx.x % 32 : threadIdx.x, step = WARP ? 32 : blockDim.x, nvec = D / N;
   if (WARP && row >= M) return;
-  V v[VPT];
+  uint4 v[VPT];
+  float f[VPT][N];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (me + i * step < nvec) v[i] = *reinterpret_cast<const V*>(x + row * ldx + (me + i * step) * N);
-  float ss = 0.f;
+  for (int i = 0; i < VPT; ++i) {
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (me + i * step < nvec) v[i] = *reinterpret_cast<const uint4*>(x + row * ldx + (me + i * step) * N);
+  }
   if (res) {
-    V r[VPT];
+    uint4 r[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-      if (me + i * step < nvec) r[i] = *reinterpret_cast<const V*>(res + row * ldres + (me + i * step) * N);
+      if (me + i * step < nvec) r[i] = *reinterpret_cast<const uint4*>(res + row * ldres + (me + i * step) * N);
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
       if (me + i * step < nvec) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[i].v[e] = from_f32<T>(to_f32(v[i].v[e]) + to_f32(r[i].v[e]));
-        *reinterpret_cast<V*>(sum_out + row * D + (me + i * step) * N) = v[i];
+        for (int c = 0; c < 4; ++c) {
+          float a[2], b[2];
+          W::unpack(word(v[i], c), a);
+          W::unpack(word(r[i], c), b);
+          a[0] += b[0];
+          if (W::PER == 2) a[1] += b[1];
+          set_word(v[i], c, W::pack(a));
+        }
+        *reinterpret_cast<uint4*>(sum_out + row * D + (me + i * step) * N) = v[i];
       }
   }
+  uint4 wv[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (me + i * step < nvec)
-#pragma unroll
-      for (int e = 0; e < N; ++e) ss = fmaf(to_f32(v[i].v[e]), to_f32(v[i].v[e]), ss);
-  const float rstd = rsqrtf((WARP ? warp_sum(ss) : block_sum_all(ss, red)) / D + eps);
-  // y is made twice, for the maximum and for q: holding it would take N registers a vector instead of 4
-  float amax[VPT];
+  for (int i = 0; i < VPT; ++i) {
+    wv[i] = make_uint4(0, 0, 0, 0);
+    if (me + i * step < nvec) wv[i] = *reinterpret_cast<const uint4*>(w + (me + i * step) * N);
+  }
+  float ss = 0.f, amax[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     amax[i] = 0.f;
-    if (me + i * step < nvec) {
-      const V wv = *reinterpret_cast<const V*>(w + (me + i * step) * N);
 #pragma unroll
-      for (int e = 0; e < N; ++e) amax[i] = fmaxf(amax[i], fabsf(to_f32(v[i].v[e]) * rstd * to_f32(wv.v[e])));
+    for (int c = 0; c < 4; ++c) {
+      float* s = f[i] + c * W::PER;
+      float g[2];
+      W::unpack(word(v[i], c), s);
+      W::unpack(word(wv[i], c), g);
+#pragma unroll
+      for (int e = 0; e < W::PER; ++e) {
+        ss = fmaf(s[e], s[e], ss);
+        s[e] *= g[e];
+        amax[i] = fmaxf(amax[i], fabsf(s[e]));
+      }
     }
   }
-  float inv = 0.f;
+  const float rstd = rsqrtf((WARP ? warp_sum(ss) : block_sum_all(ss, red)) / D + eps);
+  float factor = 0.f;
   if (block) {  // the 128 / N lanes with a block's vectors are neighbours
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
@@ -143,28 +161,32 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) norm_fp8_kernel(const T* __
     float m = amax[0];
 #pragma unroll
     for (int i = 1; i < VPT; ++i) m = fmaxf(m, amax[i]);
-    const float sc = scale_of(WARP ? warp_max(m) : block_max_all(m, red));
+    const float sc = scale_of((WARP ? warp_max(m) : block_max_all(m, red)) * rstd);
     if (me == 0) scales[row] = sc;
-    inv = 1.f / sc;
+    factor = 1.f / sc;
   }
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
     if (me + i * step < nvec) {
       const int c = (me + i * step) * N;
       if (block) {
-        const float sc = scale_of(amax[i]);
+        const float sc = scale_of(amax[i] * rstd);
         if (c % 128 == 0) scales[row * (D / 128) + c / 128] = sc;
-        inv = 1.f / sc;
+        factor = 1.f / sc;
       }
-      const V wv = *reinterpret_cast<const V*>(w + c);
-      float y[N];
+      float by = rstd * factor;
+      if (by == INFINITY) {  // rows of subnormal size, whose factors together pass f32's range
 #pragma unroll
-      for (int e = 0; e < N; ++e) y[e] = to_f32(v[i].v[e]) * rstd * to_f32(wv.v[e]) * inv;
+        for (int e = 0; e < N; ++e) f[i][e] *= rstd;
+        by = factor;
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[i][e] *= by;
       if (N == 8)
-        *reinterpret_cast<uint2*>(q + row * D + c) =
-            make_uint2(four_e4m3(y[0], y[1], y[2], y[3]), four_e4m3(y[N - 4], y[N - 3], y[N - 2], y[N - 1]));
+        *reinterpret_cast<uint2*>(q + row * D + c) = make_uint2(
+            four_e4m3(f[i][0], f[i][1], f[i][2], f[i][3]), four_e4m3(f[i][N - 4], f[i][N - 3], f[i][N - 2], f[i][N - 1]));
       else
-        *reinterpret_cast<uint32_t*>(q + row * D + c) = four_e4m3(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint32_t*>(q + row * D + c) = four_e4m3(f[i][0], f[i][1], f[i][2], f[i][3]);
     }
 }
 
@@ -181,7 +203,7 @@ int launch(const void* x, int64_t ldx, const void* res, int64_t ldres, const voi
     return (int)cudaGetLastError();
   };
   const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
-  if (!vec || nvec > 8192) {
+  if (!vec || nvec > 4096) {
     norm_fp8_any_kernel<T><<<(unsigned)M, 256, 0, st>>>((const T*)x, ldx, (const T*)res, ldres, (const T*)w, (T*)sum,
                                                         (uint8_t*)q, scales, D, block, eps);
     return (int)cudaGetLastError();
@@ -190,8 +212,7 @@ int launch(const void* x, int64_t ldx, const void* res, int64_t ldres, const voi
   if (nvec <= 64) return run(norm_fp8_kernel<T, 2, true>, 8, 256);
   if (nvec <= 128) return run(norm_fp8_kernel<T, 4, true>, 8, 256);
   if (nvec <= 512) return run(norm_fp8_kernel<T, 2, false>, 1, threads(2));
-  if (nvec <= 1024) return run(norm_fp8_kernel<T, 4, false>, 1, threads(4));
-  return run(norm_fp8_kernel<T, 8, false>, 1, threads(8));
+  return run(norm_fp8_kernel<T, 4, false>, 1, threads(4));
 }
 
 }  // namespace

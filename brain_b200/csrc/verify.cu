@@ -13,10 +13,8 @@
 //
 // Bound by memory: one row of p a sequence and one of q where a token is refused; the rows of the other
 // positions are touched at one value each. A cluster of CTAs shares a row, as many as fill the GPU at this
-// batch; each warp sums one contiguous segment with coalesced loads of single values (any alignment, eight of p
-// and of q in flight a lane), and only the segment that holds the border is read again, out of cache. p alone
-// is summed only where p - q is empty. Loads of 4 bytes cost nothing here: a warp's are whole 128-byte lines,
-// and conversions to 64 bits, not loads, take the most issue slots.
+// batch; each warp sums one contiguous segment, with 16-byte loads where the rows lie alike, and only the
+// segment that holds the border is read again, out of cache. p alone is summed only where p - q is empty.
 #include "elem.cuh"
 
 using namespace brain;
@@ -44,13 +42,11 @@ __device__ __forceinline__ float weight(float v) { return v > 0.f && v < INFINIT
 template <typename T>
 struct Mass {
   const T *p, *q;
-  int64_t hole;
-  __device__ __forceinline__ double operator()(int j, T pj, T qj) const {
-    const float a = weight(to_f32(pj));
-    const float b = q ? weight(to_f32(qj)) : 0.f;
+  int hole;
+  __device__ __forceinline__ double operator()(int j) const {
+    const float a = weight(to_f32(p[j])), b = q ? weight(to_f32(q[j])) : 0.f;
     return a > b && j != hole ? (double)a - (double)b : 0.0;
   }
-  __device__ __forceinline__ double operator()(int j) const { return (*this)(j, p[j], q ? q[j] : T(0.f)); }
 };
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
@@ -59,57 +55,105 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
-// Sum of [from, to) by one warp.
-template <typename T>
-__device__ __forceinline__ double segment_sum(const Mass<T>& mass, int from, int to) {
-  constexpr int U = 8;
+// Sum of [from, to) of p - q (Q) or p by one warp; `from` lies on a 16-byte boundary of both rows where vec is set.
+template <typename T, bool Q>
+__device__ __forceinline__ double segment_rows(const T* p, const T* q, int from, int to, bool vec) {
+  using W = Words<T>;
+  constexpr int U = 4;
   const int lane = threadIdx.x % 32;
   double s = 0;
-  int j = from + lane;
-  for (; j + (U - 1) * 32 < to; j += U * 32) {
-    T a[U], b[U];
+  const auto add = [&](float pj, float qj) {
+    const float a = weight(pj);
+    if (Q) {
+      const float b = weight(qj);
+      if (a > b) s += (double)a - (double)b;
+    } else {
+      s += (double)a;
+    }
+  };
+  int j = from;
+  if (vec)
+    for (; j + U * 32 * W::N <= to; j += U * 32 * W::N) {
+      uint4 a[U], b[U];
 #pragma unroll
-    for (int c = 0; c < U; ++c) a[c] = mass.p[j + c * 32];
+      for (int c = 0; c < U; ++c) a[c] = *reinterpret_cast<const uint4*>(p + j + (c * 32 + lane) * W::N);
+      if (Q)
 #pragma unroll
-    for (int c = 0; c < U; ++c) b[c] = mass.q ? mass.q[j + c * 32] : T(0.f);
+        for (int c = 0; c < U; ++c) b[c] = *reinterpret_cast<const uint4*>(q + j + (c * 32 + lane) * W::N);
 #pragma unroll
-    for (int c = 0; c < U; ++c) s += mass(j + c * 32, a[c], b[c]);
+      for (int c = 0; c < U; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[2], g[2] = {0.f, 0.f};
+          W::unpack(word(a[c], i), f);
+          if (Q) W::unpack(word(b[c], i), g);
+#pragma unroll
+          for (int e = 0; e < W::PER; ++e) add(f[e], g[e]);
+        }
+    }
+  for (j += lane; j + 7 * 32 < to; j += 8 * 32) {
+    T a[8], b[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) a[c] = p[j + c * 32];
+    if (Q)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) b[c] = q[j + c * 32];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) add(to_f32(a[c]), Q ? to_f32(b[c]) : 0.f);
   }
-  for (; j < to; j += 32) s += mass(j);
+  for (; j < to; j += 32) add(to_f32(p[j]), Q ? to_f32(q[j]) : 0.f);
   return warp_sum_f64(s);
 }
 
-__device__ __forceinline__ double ld_dsmem_f64(uint32_t addr) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
-  return v;
+template <typename T>
+__device__ __forceinline__ double segment_sum(const Mass<T>& m, int from, int to, bool vec) {
+  if (m.q) return segment_rows<T, true>(m.p, m.q, from, to, vec);
+  double s = segment_rows<T, false>(m.p, nullptr, from, min(max(m.hole, from), to), vec);
+  if (m.hole < from) return segment_rows<T, false>(m.p, nullptr, from, to, vec);
+  if (m.hole < to) s += segment_rows<T, false>(m.p, nullptr, m.hole + 1, to, false);
+  return s;
 }
 
-// The first of n sums, counted on from `base`, with which the running sum exceeds the goal; the last with any
-// mass where none does; -1 where none has any. `base` becomes the sum before it.
+// By one warp: the first of n sums, counted on from `base`, with which the running sum exceeds the goal; the last
+// with any mass where none does; -1 where none has any. `base` becomes the sum before it.
 template <typename F>
 __device__ int crossing(F sum, int n, double goal, double& base) {
-  int at = -1;
-  double run = base;
-  for (int i = 0; i < n; ++i) {
-    const double s = sum(i);
-    if (s > 0) {
-      at = i;
-      base = run;
-      if (run + s > goal) break;
-    }
-    run += s;
+  const int lane = threadIdx.x % 32, each = (n + 31) / 32, from = min(lane * each, n), to = min(from + each, n);
+  double mine = 0;
+  for (int i = from; i < to; ++i) mine += sum(i);
+  double run = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const double v = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += v;
   }
-  return at;
+  const unsigned some = __ballot_sync(0xffffffffu, mine > 0), over = __ballot_sync(0xffffffffu, mine > 0 && base + run > goal);
+  if (!some) return -1;
+  const int pick = over ? __ffs(over) - 1 : 31 - __clz(some);
+  int at = 0;
+  double before = base + (run - mine), r = before;
+  if (lane == pick)
+    for (int i = from; i < to; ++i) {
+      const double s = sum(i);
+      if (s > 0) {
+        at = i;
+        before = r;
+        if (r + s > goal) break;
+      }
+      r += s;
+    }
+  base = __shfl_sync(0xffffffffu, before, pick);
+  return __shfl_sync(0xffffffffu, at, pick);
 }
 
 // A cluster per sequence: rank r takes the r-th share of the vocabulary, its warps contiguous segments of it.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
-  __shared__ double seg[kWarps], all[kMaxCluster * kWarps];
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(VerifyArgs a) {
+  __shared__ double all[2][kMaxCluster * kWarps], seg[kWarps];
   __shared__ int s_n, s_at;
-  __shared__ double s_base, s_goal;
+  __shared__ double s_goal;
   const int b = blockIdx.y, rank = blockIdx.x, ranks = gridDim.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const T* pb = (const T*)a.p + b * a.p_seq;
   const T* qb = a.q ? (const T*)a.q + b * a.q_seq : nullptr;
   const int64_t* drafted = a.drafted + (int64_t)b * a.K;
@@ -139,73 +183,53 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
   __syncthreads();
   const int n = s_n;
   const bool refused = n < len;
-  Mass<T> mass{pb + n * a.p_pos, refused && qb ? qb + n * a.q_pos : nullptr, refused && !qb ? drafted[n] : -1};
+  Mass<T> mass{pb + n * a.p_pos, refused && qb ? qb + n * a.q_pos : nullptr, -1};
+  if (refused && !qb && drafted[n] >= 0 && drafted[n] < a.V) mass.hole = (int)drafted[n];
+  const bool vec = ((reinterpret_cast<uintptr_t>(mass.p) | reinterpret_cast<uintptr_t>(mass.q)) & 15) == 0;
   const int parts = ranks * kWarps, size = ((a.V + parts - 1) / parts + 31) & ~31;
-  const auto start = [&](int part) { return min((int64_t)part * size, (int64_t)a.V); };
+  const auto start = [&](int part) { return (int)min((int64_t)part * size, (int64_t)a.V); };
+  const int part = rank * kWarps + warp;
+  if (ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all ranks run
   // twice at most: p - q, then p where that is empty
-  for (bool again = false;; again = true) {
-    const int part = rank * kWarps + warp;
-    const double s = segment_sum(mass, (int)start(part), (int)start(part + 1));
-    if (lane == 0) seg[warp] = s;
-    if (ranks > 1)
+  int pass = 0;
+  for (;; pass = 1) {
+    const double s = segment_sum(mass, start(part), start(part + 1), vec);
+    if (ranks > 1) {
+      if (lane < ranks)
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&all[pass][part]), lane)), "d"(s) : "memory");
+      __syncwarp();
       cluster_sync();
-    else
+    } else {
+      if (lane == 0) all[pass][part] = s;
       __syncthreads();
-    for (int i = threadIdx.x; i < parts; i += kThreads)
-      all[i] = ranks > 1 ? ld_dsmem_f64(mapa_shared(smem_u32(seg + i % kWarps), i / kWarps)) : seg[i];
-    if (ranks > 1)
-      cluster_sync();  // the segments have been read: they may be written again, or the CTA may leave
-    else
-      __syncthreads();
-    if (warp == 0) {
-      double total = 0;
-      for (int i = lane; i < parts; i += 32) total += all[i];
-      total = warp_sum_f64(total);
-      if (lane == 0) s_goal = total;
     }
-    __syncthreads();
-    if (s_goal > 0 || !refused || again) break;
+    // every warp finds the same border
+    double total = 0;
+    for (int i = lane; i < parts; i += 32) total += all[pass][i];
+    total = warp_sum_f64(total);
+    if (warp == 0 && lane == 0) s_goal = total * (double)u[a.K];
+    if (total > 0 || !refused || pass) break;
     mass.q = nullptr;
     mass.hole = -1;
   }
-  if (threadIdx.x == 0) {
-    s_goal *= (double)u[a.K];
-    s_base = 0;
-    s_at = crossing([&](int i) { return all[i]; }, parts, s_goal, s_base);
-  }
   __syncthreads();
-  int at = s_at;
+  const double goal = s_goal;
+  double base = 0;
+  int at = crossing([&](int i) { return all[pass][i]; }, parts, goal, base);
   // the rank that holds the segment finds the id, rank 0 where there is none
   if (at >= 0 ? at / kWarps != rank : rank != 0) return;
-  const double goal = s_goal;
-  double base = s_base;
   if (at >= 0) {
-    const int lo = (int)start(at), hi = (int)start(at + 1), sub = (hi - lo + kWarps - 1) / kWarps;
+    const int lo = start(at), hi = start(at + 1), sub = (hi - lo + kWarps - 1) / kWarps;
     const int from = min(lo + warp * sub, hi), to = min(from + sub, hi);
-    const double s = segment_sum(mass, from, to);
-    __syncthreads();
+    const double s = segment_sum(mass, from, to, false);
     if (lane == 0) seg[warp] = s;
     __syncthreads();
-    const int w = crossing([&](int i) { return seg[i]; }, kWarps, goal, base);
-    // w < 0: its mass is there, but not in any part of it, which only rounding could do
-    const int wfrom = min(lo + max(w, 0) * sub, hi), wto = min(wfrom + sub, hi);
-    if (warp == 0) {  // a lane takes adjacent ids
-      const int each = (wto - wfrom + 31) / 32, f = min(wfrom + lane * each, wto), t = min(f + each, wto);
-      double mine = 0;
-      for (int j = f; j < t; ++j) mine += mass(j);
-      double run = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const double v = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += v;
-      }
-      const unsigned some = __ballot_sync(0xffffffffu, mine > 0), over = __ballot_sync(0xffffffffu, mine > 0 && base + run > goal);
-      const int pick = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : 0;
-      if (lane == pick) {
-        double before = base + (run - mine);
-        const int j = crossing([&](int i) { return mass(f + i); }, t - f, goal, before);
-        s_at = f + max(j, 0);
-      }
+    if (warp == 0) {
+      // a segment with mass has a part with mass: the sums are of the same non-negative numbers
+      const int w = max(crossing([&](int i) { return seg[i]; }, kWarps, goal, base), 0);
+      const int wfrom = min(lo + w * sub, hi), wto = min(wfrom + sub, hi);
+      const int j = crossing([&](int i) { return mass(wfrom + i); }, wto - wfrom, goal, base);
+      if (lane == 0) s_at = wfrom + max(j, 0);
     }
     __syncthreads();
     at = s_at;
