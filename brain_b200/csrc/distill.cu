@@ -11,8 +11,17 @@
 // factor), the gradient a second pass over the same row. One id may occur twice: its entries add up in
 // their order, by the thread of the first, so the result is the same every time.
 //
-// Bound by memory: the logits once for the loss; once in and once out for the gradient. A CTA takes a row,
-// and reads it a second time for the gradient right after the first, while it is still in L2.
+// Bound by memory: the logits once for the loss; once in and once out for the gradient. Three kernels:
+//   loss, or loss and gradient: a cluster of CTAs holds a row in shared memory, brought by bulk copies in pieces
+//     that are summed as they land. The ranks exchange their maxima and sums, and for the gradient turn what they
+//     hold into it in place and copy it back: one read, one write. Two to four CTAs share an SM, so that one
+//     computes while others copy.
+//   gradient alone (the backward pass of autograd, from the kept log-sum-exp): a stream, a CTA a piece of a row.
+//   rows that 16 x 96 KB do not hold (and gradients that lie otherwise on 16 bytes than their logits): a CTA a row,
+//     read twice.
+#include <algorithm>
+#include <type_traits>
+
 #include "elem.cuh"
 
 using namespace brain;
@@ -228,6 +237,330 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a) {
       dz[top.id[i]] = from_f32<T>(g * (ex2(fmaf(top.zk[i], factor, -lse2)) - total[i]));
 }
 
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kHold = 256;            // threads of a holding CTA
+constexpr int kPiece = 8192;          // bytes of a bulk copy
+constexpr int kMaxHold = 96 * 1024;   // bytes of a row in one CTA at most
+constexpr int kHoldTarget = 64 * 1024;  // and as many as leave room for three CTAs an SM
+constexpr int kMaxCluster = 16;
+
+// Where a row's 16-byte vectors begin, and which of them a rank of `ranks` takes; single values at the ends belong
+// to the first and the last rank.
+template <typename T>
+struct Slice {
+  int head, nv, v0, v1;
+  __device__ __forceinline__ Slice(const T* z, int V, int rank, int ranks) {
+    constexpr int N = 16 / sizeof(T);
+    head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T)));
+    nv = (V - head) / N;
+    const int per = (nv + ranks - 1) / ranks;
+    v0 = min(rank * per, nv);
+    v1 = min(v0 + per, nv);
+  }
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(kHold) distill_hold_kernel(DistillArgs a, int ranks) {
+  using W = Words<T>;
+  extern __shared__ __align__(16) uint8_t hold[];
+  __shared__ float red[32];
+  __shared__ float share[3][kMaxCluster];
+  __shared__ __align__(8) uint64_t bars[kMaxHold / kPiece];
+  __shared__ int abort_flag;
+  const int64_t row = blockIdx.x / ranks;
+  const int rank = blockIdx.x % ranks, tid = threadIdx.x;
+  const T* z = (const T*)a.z + row * a.ldz;
+  const Slice<T> sl(z, a.V, rank, ranks);
+  const int bytes = (sl.v1 - sl.v0) * 16, pieces = (bytes + kPiece - 1) / kPiece;
+  const uint32_t sbase = smem_u32(hold);
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < pieces; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    fence_barrier_init();
+    for (int i = 0; i < pieces; ++i) {
+      const int n = min(kPiece, bytes - i * kPiece);
+      mbar_arrive_expect_tx(smem_u32(&bars[i]), n);
+      bulk_load(sbase + i * kPiece, reinterpret_cast<const uint8_t*>(z + sl.head) + (int64_t)sl.v0 * 16 + i * kPiece, n,
+                smem_u32(&bars[i]));
+    }
+  }
+
+  // the teacher's entries: p of all of them; z and the loss's terms of those in this rank's part
+  const int held = (bytes + 15) & ~15;
+  float* p = reinterpret_cast<float*>(hold + held);
+  float* zk = p + a.k;
+  int* id = reinterpret_cast<int*>(p + 2 * a.k);
+  float top = -INFINITY;
+  bool nan = false;
+  for (int i = tid; i < a.k; i += kHold) {
+    const int64_t j = a.id[row * a.k + i];
+    const float t = a.t[row * a.k + i] * a.inv_t;
+    if (j >= a.V) set_status(BRAIN_ERR_BOUNDS, 711);
+    const bool on = j >= 0 && j < a.V && t != -INFINITY;
+    id[i] = on ? (int)j : -1;
+    p[i] = t;
+    if (on) {
+      top = fmaxf(top, t);
+      nan |= t != t;
+    }
+  }
+  const float factor = a.inv_t * kLog2e;
+  float m = -INFINITY, s = 0.f;
+  // the single values at the ends, one a thread
+  int end = -1;
+  if (rank == 0 && tid < sl.head) end = tid;
+  const int tail = sl.head + sl.nv * W::N;
+  if (rank == ranks - 1 && tid >= 32 && tid - 32 < a.V - tail) end = tail + tid - 32;
+  float zend = 0.f;
+  if (end >= 0) {
+    zend = to_f32(z[end]);
+    const float f = zend * factor;
+    merge(m, s, f, f == -INFINITY ? 0.f : ex2(f - f));
+  }
+  top = block_max_all(top, red);
+  const bool any = __syncthreads_or(top > -INFINITY || nan);  // (the barriers are set up, too)
+  float sum = 0.f;
+  for (int i = tid; i < a.k; i += kHold) {
+    p[i] = id[i] >= 0 ? expf(p[i] - top) : 0.f;
+    sum += p[i];
+  }
+  sum = block_sum_all(sum, red);
+
+  // ---- the running maximum and sum, over the pieces as they land
+  bool ok = true;
+  for (int c = 0; c < pieces; ++c) {
+    ok = ok && mbar_wait(smem_u32(&bars[c]), 0, BRAIN_ERR_TIMEOUT_FULL, 712, &abort_flag);
+    const int stop = min((c + 1) * kPiece, bytes);
+    constexpr int U = kPiece / (kHold * 16);
+    uint4 v[U];
+    float f[U][W::N], lm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = c * kPiece + (u * kHold + tid) * 16;
+      const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+      v[u] = at < stop ? *reinterpret_cast<const uint4*>(hold + at) : make_uint4(none, none, none, none);  // -inf
+#pragma unroll
+      for (int i = 0; i < 4; ++i) W::unpack(word(v[u], i), f[u] + i * W::PER);
+#pragma unroll
+      for (int e = 0; e < W::N; ++e) lm = fmaxf(lm, f[u][e]);
+    }
+    lm *= factor;
+    const float top2 = fmaxf(m, lm), base = top2 == -INFINITY ? 0.f : top2;
+    s *= m == -INFINITY ? 1.f : ex2(m - base);
+    m = top2;
+    float ls[2] = {};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < W::N; ++e) ls[e & 1] += ex2(fmaf(f[u][e], factor, -base));
+    s += ls[0] + ls[1];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    merge(m, s, m2, s2);
+  }
+  __shared__ float wm[kHold / 32], ws[kHold / 32];
+  if (tid % 32 == 0) {
+    wm[tid / 32] = m;
+    ws[tid / 32] = s;
+  }
+  float kl = 0.f;
+  for (int i = tid; i < a.k; i += kHold) {
+    const int j = id[i];
+    if (j < 0) continue;
+    const int v = j < sl.head || j >= tail ? -1 : (j - sl.head) / W::N;
+    const bool mine = j < sl.head ? rank == 0 : j >= tail ? rank == ranks - 1 : v >= sl.v0 && v < sl.v1;
+    const float pi = p[i] / sum;
+    p[i] = pi;
+    if (!mine) {
+      id[i] = -1 - j;  // another rank's
+      continue;
+    }
+    zk[i] = to_f32(v < 0 ? z[j] : reinterpret_cast<const T*>(hold)[j - sl.head - sl.v0 * W::N]);
+    if (pi != 0.f) kl += pi * (logf(pi) - zk[i] * a.inv_t);
+  }
+  kl = block_sum_all(kl, red);
+  if (ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all ranks run
+  if (tid < 32) {
+    m = tid < kHold / 32 ? wm[tid] : -INFINITY;
+    s = tid < kHold / 32 ? ws[tid] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      merge(m, s, m2, s2);
+    }
+    if (tid < ranks) {
+      const float out[3] = {m, s, kl};
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&share[i][rank]), tid)), "f"(out[i])
+                     : "memory");
+    }
+    __syncwarp();
+  }
+  if (ranks > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  m = share[0][0];
+  s = share[1][0];
+  kl = share[2][0];
+  for (int r = 1; r < ranks; ++r) {
+    merge(m, s, share[0][r], share[1][r]);
+    kl += share[2][r];
+  }
+  const float lse = (m + log2f(s)) * kLn2;
+  if (rank == 0 && tid == 0) {
+    a.loss[row] = any ? a.temp * a.temp * (kl + lse) : 0.f;
+    if (a.lse) a.lse[row] = lse;
+  }
+  if (!GRAD) return;
+
+  // ---- the gradient, in place
+  T* dz = (T*)a.dz + row * a.lddz;
+  const float g = any ? (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * (a.inv_n ? *a.inv_n : 1.f) * a.temp : 0.f;
+  const float lse2 = lse * kLog2e;
+  for (int at = tid * 16; at < bytes; at += kHold * 16) {
+    uint4 v = *reinterpret_cast<const uint4*>(hold + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[2];
+      W::unpack(word(v, i), f);
+#pragma unroll
+      for (int e = 0; e < W::PER; ++e) f[e] = any ? g * ex2(fmaf(f[e], factor, -lse2)) : 0.f;
+      set_word(v, i, W::pack(f));
+    }
+    *reinterpret_cast<uint4*>(hold + at) = v;
+  }
+  if (end >= 0) dz[end] = from_f32<T>(any ? g * ex2(fmaf(zend, factor, -lse2)) : 0.f);
+  __syncthreads();
+  // the first entry with an id takes the sum of all that share it, in their order
+  for (int i = tid; i < a.k; i += kHold) {
+    const int j = id[i];
+    if (j < 0) continue;
+    float total = 0.f;
+    bool first = true;
+    for (int c = 0; c < a.k; ++c)
+      if (id[c] == j) {
+        if (c < i) first = false;
+        total += p[c];
+      }
+    if (!first) continue;
+    const T d = from_f32<T>(g * (ex2(fmaf(zk[i], factor, -lse2)) - total));
+    if (j < sl.head || j >= tail)
+      dz[j] = d;
+    else
+      reinterpret_cast<T*>(hold)[j - sl.head - sl.v0 * W::N] = d;
+  }
+  fence_proxy_async();  // what was written here is read by the copies
+  __syncthreads();
+  if (tid == 0 && bytes > 0) {
+    uint8_t* to = reinterpret_cast<uint8_t*>(dz + sl.head) + (int64_t)sl.v0 * 16;
+    for (int i = 0; i < pieces; ++i) bulk_store(to + i * kPiece, sbase + i * kPiece, min(kPiece, bytes - i * kPiece));
+    tma_store_commit();
+    tma_store_wait_read<0>();  // the CTA's memory stays until it has been read
+  }
+}
+
+// The gradient from the kept log-sum-exp: a CTA a piece of a row, a vector of four a thread at a time.
+template <typename T>
+__global__ void __launch_bounds__(kHold) distill_grad_kernel(DistillArgs a, int ranks) {
+  using W = Words<T>;
+  constexpr int U = 4;
+  extern __shared__ float entries[];
+  __shared__ float red[32];
+  const int64_t row = blockIdx.x / ranks;
+  const int tid = threadIdx.x, rank = blockIdx.x % ranks;
+  const T* z = (const T*)a.z + row * a.ldz;
+  T* dz = (T*)a.dz + row * a.lddz;
+  const Slice<T> sl(z, a.V, rank, ranks);
+  const uint4* zv = reinterpret_cast<const uint4*>(z + sl.head);
+  uint4* dv = reinterpret_cast<uint4*>(dz + sl.head);
+  // the first vectors are on their way while the entries are looked at
+  uint4 v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (sl.v0 + u * kHold + tid < sl.v1) v[u] = zv[sl.v0 + u * kHold + tid];
+  float* p = entries;
+  float* zk = p + a.k;
+  int* id = reinterpret_cast<int*>(p + 2 * a.k);
+  float top = -INFINITY;
+  bool nan = false;
+  const int tail = sl.head + sl.nv * W::N;
+  for (int i = tid; i < a.k; i += kHold) {
+    const int64_t j = a.id[row * a.k + i];
+    const float t = a.t[row * a.k + i] * a.inv_t;
+    const bool on = j >= 0 && j < a.V && t != -INFINITY;
+    const int at = (int)(on ? j : 0), w = (at - sl.head) / W::N;
+    const bool mine = on && (at < sl.head ? rank == 0 : at >= tail ? rank == ranks - 1 : w >= sl.v0 && w < sl.v1);
+    id[i] = on ? (mine ? at : -1 - at) : INT32_MIN;
+    p[i] = t;
+    zk[i] = mine ? to_f32(z[at]) : 0.f;
+    if (on) {
+      top = fmaxf(top, t);
+      nan |= t != t;
+    }
+  }
+  top = block_max_all(top, red);
+  const bool any = __syncthreads_or(top > -INFINITY || nan);
+  float sum = 0.f;
+  for (int i = tid; i < a.k; i += kHold) {
+    p[i] = id[i] != INT32_MIN ? expf(p[i] - top) : 0.f;
+    sum += p[i];
+  }
+  sum = block_sum_all(sum, red);
+  const float factor = a.inv_t * kLog2e, lse2 = a.lse[row] * kLog2e;
+  const float g = any ? (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * (a.inv_n ? *a.inv_n : 1.f) * a.temp : 0.f;
+  for (int at = sl.v0; at < sl.v1; at += U * kHold) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = at + u * kHold + tid;
+      if (i >= sl.v1) continue;
+      uint4 o;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float f[2];
+        W::unpack(word(v[u], c), f);
+#pragma unroll
+        for (int e = 0; e < W::PER; ++e) f[e] = any ? g * ex2(fmaf(f[e], factor, -lse2)) : 0.f;
+        set_word(o, c, W::pack(f));
+      }
+      dv[i] = o;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (at + (U + u) * kHold + tid < sl.v1) v[u] = zv[at + (U + u) * kHold + tid];
+  }
+  int end = -1;
+  if (rank == 0 && tid < sl.head) end = tid;
+  if (rank == ranks - 1 && tid >= 32 && tid - 32 < a.V - tail) end = tail + tid - 32;
+  if (end >= 0) dz[end] = from_f32<T>(any ? g * ex2(fmaf(to_f32(z[end]), factor, -lse2)) : 0.f);
+  __syncthreads();
+  for (int i = tid; i < a.k; i += kHold) {
+    const int j = id[i];
+    if (j < 0) continue;
+    float total = 0.f;
+    bool first = true;
+    for (int c = 0; c < a.k; ++c)
+      if (id[c] == j) {
+        if (c < i) first = false;
+        total += p[c] / sum;
+      }
+    if (first) dz[j] = from_f32<T>(g * (ex2(fmaf(zk[i], factor, -lse2)) - total));
+  }
+}
+
 // Rows that have an entry, counted before the gradient of a mean is written: a warp a row.
 __global__ void distill_count_kernel(const float* __restrict__ t, const int64_t* __restrict__ id, int64_t M, int k, int V,
                                      int* __restrict__ count) {
@@ -262,8 +595,44 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __res
   }
 }
 
+template <typename T, bool GRAD>
+int launch_hold(const DistillArgs& a, int64_t M, int ranks, int held, cudaStream_t st) {
+  const auto kernel = distill_hold_kernel<T, GRAD>;
+  const int smem = held + a.k * 12;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxHold + 16 + kMaxTop * 12);
+  if (e == cudaSuccess && ranks > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(M * ranks));
+  cfg.blockDim = dim3(kHold);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ranks;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, a, ranks);
+}
+
 template <typename T>
 int launch(const DistillArgs& a, int64_t M, cudaStream_t st) {
+  const int64_t bytes = (int64_t)a.V * sizeof(T);
+  const bool alike = !a.dz || ((reinterpret_cast<uintptr_t>(a.z) ^ reinterpret_cast<uintptr_t>(a.dz)) & 15) == 0 &&
+                                  ((a.ldz - a.lddz) * sizeof(T)) % 16 == 0;
+  if (alike && !a.loss) {
+    // pieces of 64 KB: short enough for an even end, long enough to hide the look at the entries
+    const int ranks = (int)std::min<int64_t>((bytes + 65535) / 65536, INT32_MAX / M);
+    distill_grad_kernel<T><<<(unsigned)(M * ranks), kHold, a.k * 12, st>>>(a, ranks);
+    return (int)cudaGetLastError();
+  }
+  int ranks = 1;
+  while (ranks < kMaxCluster && bytes > ranks * (int64_t)kHoldTarget) ranks *= 2;
+  const int64_t held = ((bytes / 16 + ranks) / ranks) * 16;
+  if (alike && a.loss && held <= kMaxHold && M * ranks <= INT32_MAX)
+    return a.dz ? launch_hold<T, true>(a, M, ranks, (int)held, st) : launch_hold<T, false>(a, M, ranks, (int)held, st);
   const size_t smem = (size_t)a.k * 16;
   const unsigned grid = (unsigned)M;
   if (a.loss && a.dz)

@@ -91,15 +91,15 @@ __device__ __forceinline__ double segment_rows(const T* p, const T* q, int from,
           for (int e = 0; e < W::PER; ++e) add(f[e], g[e]);
         }
     }
-  for (j += lane; j + 7 * 32 < to; j += 8 * 32) {
-    T a[8], b[8];
+  for (j += lane; j + 15 * 32 < to; j += 16 * 32) {
+    T a[16], b[16];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) a[c] = p[j + c * 32];
+    for (int c = 0; c < 16; ++c) a[c] = p[j + c * 32];
     if (Q)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) b[c] = q[j + c * 32];
+      for (int c = 0; c < 16; ++c) b[c] = q[j + c * 32];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) add(to_f32(a[c]), Q ? to_f32(b[c]) : 0.f);
+    for (int c = 0; c < 16; ++c) add(to_f32(a[c]), Q ? to_f32(b[c]) : 0.f);
   }
   for (; j < to; j += 32) add(to_f32(p[j]), Q ? to_f32(q[j]) : 0.f);
   return warp_sum_f64(s);
@@ -239,10 +239,10 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(VerifyArgs a) {
   if (threadIdx.x == 0) a.count[b] = n;
 }
 
-// CTAs a sequence: as many as keep about three of them on every SM, no more than leave a warp 128 ids.
+// CTAs a sequence: as many as run at once (two an SM), no more than leave a warp 128 ids.
 int plan_ranks(int64_t B, int V) {
   int c = 1;
-  while (c < kMaxCluster && B * c * 2 <= 3 * brain_host::num_sms() && V / (c * 2 * kWarps) >= 128) c *= 2;
+  while (c < kMaxCluster && B * c * 2 <= 2 * brain_host::num_sms() && V / (c * 2 * kWarps) >= 128) c *= 2;
   return c;
 }
 
