@@ -11,14 +11,10 @@
 // factor), the gradient a second pass over the same row. One id may occur twice: its entries add up in
 // their order, by the thread of the first, so the result is the same every time.
 //
-// Bound by memory: the logits once for the loss; once in and once out for the gradient. Three kernels:
-//   loss, or loss and gradient: a cluster of CTAs holds a row in shared memory, brought by bulk copies in pieces
-//     that are summed as they land. The ranks exchange their maxima and sums, and for the gradient turn what they
-//     hold into it in place and copy it back: one read, one write. Two to four CTAs share an SM, so that one
-//     computes while others copy.
-//   gradient alone (the backward pass of autograd, from the kept log-sum-exp): a stream, a CTA a piece of a row.
-//   rows that 16 x 96 KB do not hold (and gradients that lie otherwise on 16 bytes than their logits): a CTA a row,
-//     read twice.
+// Bound by memory: the logits once for the loss; once in and once out for the gradient. A CTA takes a row and, for
+// the gradient, reads it again right after the first pass, out of L2; the backward pass of autograd has the
+// log-sum-exp and streams pieces of rows. Exponentials are not what bounds: without them 2048 x 128256 takes 243 us
+// in place of 254.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,7 +24,6 @@ using namespace brain;
 
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kMaxTop = 1024;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -40,10 +35,12 @@ struct DistillArgs {
   const int64_t* id;     // [M, k]
   float* loss;           // [M], null in the backward pass
   float* lse;            // [M], written with the loss, read in the backward pass
+  float* counts;         // [M], 1 where the row has an entry, else 0; may be null
   void* dz;              // null for the loss alone
   int64_t lddz;
   const float* grad;     // upstream gradient: a scalar, or one a row
-  const float* inv_n;    // 1 / rows that count, null: 1
+  const int* n;          // numbers of rows that count, to be added up and divided by; null: no division
+  int parts;             // how many
   int grad_rows;
   int k, V;
   float inv_t, temp;     // 1 / T, T
@@ -62,187 +59,7 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
   m = top;
 }
 
-// The kept entries of a row, made once by its CTA.
-struct Top {
-  float* p;        // [k] probability; after dedup() 0 where an earlier entry has the same id
-  float* zk;       // [k] z at the id, as given
-  int* id;         // [k] -1: none
-  float kl;        // sum_i p_i (log p_i - z_i / T): the loss is T^2 (kl + lse)
-  bool any;
-};
-
-template <typename T>
-__device__ Top load_top(const DistillArgs& a, int64_t row, const T* z, float* smem, float* red) {
-  Top r;
-  r.p = smem;
-  r.zk = smem + a.k;
-  r.id = reinterpret_cast<int*>(smem + 2 * a.k);
-  float top = -INFINITY;
-  bool nan = false;
-  for (int i = threadIdx.x; i < a.k; i += kThreads) {
-    const int64_t j = a.id[row * a.k + i];
-    float t = a.t[row * a.k + i] * a.inv_t;
-    if (j >= a.V) set_status(BRAIN_ERR_BOUNDS, 710);
-    const bool on = j >= 0 && j < a.V && t != -INFINITY;
-    r.id[i] = on ? (int)j : -1;
-    r.p[i] = t;
-    r.zk[i] = on ? to_f32(z[j]) : 0.f;
-    if (on) {
-      top = fmaxf(top, t);
-      nan |= t != t;
-    }
-  }
-  top = block_max_all(top, red);
-  // a NaN among the entries leaves a maximum of the others (or none); the sums below carry it on
-  r.any = __syncthreads_or(top > -INFINITY || nan);
-  float sum = 0.f;
-  for (int i = threadIdx.x; i < a.k; i += kThreads) {
-    r.p[i] = r.id[i] >= 0 ? expf(r.p[i] - top) : 0.f;
-    sum += r.p[i];
-  }
-  sum = block_sum_all(sum, red);
-  float kl = 0.f;
-  for (int i = threadIdx.x; i < a.k; i += kThreads)
-    if (r.id[i] >= 0) {
-      const float p = r.p[i] / sum;
-      r.p[i] = p;
-      if (p != 0.f) kl += p * (logf(p) - r.zk[i] * a.inv_t);
-    }
-  r.kl = block_sum_all(kl, red);
-  return r;
-}
-
-// The first entry with an id takes the sum of all that share it, in their order.
-__device__ void dedup(const Top& r, int k, float* total) {
-  for (int i = threadIdx.x; i < k; i += kThreads) {
-    const int id = r.id[i];
-    float t = 0.f;
-    bool first = id >= 0;
-    for (int j = 0; j < k; ++j)
-      if (r.id[j] == id) {
-        if (j < i) first = false;
-        t += r.p[j];
-      }
-    total[i] = first ? t : -1.f;
-  }
-}
-
-// f(index, value) over the row: 16-byte loads over the aligned middle, four in flight, single values at the ends.
-template <typename T, typename F8, typename F1>
-__device__ __forceinline__ void for_row(const T* z, int V, F8 vec, F1 one) {
-  constexpr int N = Vec16<T>::N;
-  const int head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T)));
-  const int nv = (V - head) / N;
-  const Vec16<T>* zv = reinterpret_cast<const Vec16<T>*>(z + head);
-  for (int i = threadIdx.x; i < nv; i += kThreads * 4) {
-    Vec16<T> v[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (i + c * kThreads < nv) v[c] = zv[i + c * kThreads];
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (i + c * kThreads < nv) vec(head + (i + c * kThreads) * N, v[c]);
-  }
-  const int tail = head + nv * N;
-  for (int i = threadIdx.x; i < head + V - tail; i += kThreads) {
-    const int j = i < head ? i : tail + i - head;
-    one(j, z[j]);
-  }
-}
-
-// LSE: find the row's log-sum-exp (the forward pass), else take a.lse. GRAD: write the gradient.
-template <typename T, bool LSE, bool GRAD>
-__global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a) {
-  extern __shared__ float smem[];
-  __shared__ float red[32], red2[32];
-  constexpr int N = Vec16<T>::N;
-  const int64_t row = blockIdx.x;
-  const T* z = (const T*)a.z + row * a.ldz;
-  Top top = load_top<T>(a, row, z, smem, red);
-  const float factor = a.inv_t * kLog2e;
-  float lse;
-  if (LSE) {
-    float m = -INFINITY, s = 0.f;
-    for_row<T>(
-        z, a.V,
-        [&](int, const Vec16<T>& v) {
-          float f[N], lm = -INFINITY, ls = 0.f;
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            f[j] = to_f32(v.v[j]) * factor;
-            lm = fmaxf(lm, f[j]);
-          }
-          const float base = lm == -INFINITY ? 0.f : lm;
-#pragma unroll
-          for (int j = 0; j < N; ++j) ls += ex2(f[j] - base);
-          merge(m, s, lm, ls);
-        },
-        [&](int, T v) {
-          const float f = to_f32(v) * factor;
-          merge(m, s, f, f == -INFINITY ? 0.f : ex2(f - f));
-        });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      merge(m, s, m2, s2);
-    }
-    const int w = threadIdx.x / 32, l = threadIdx.x % 32;
-    __syncthreads();
-    if (l == 0) {
-      red[w] = m;
-      red2[w] = s;
-    }
-    __syncthreads();
-    m = l < kThreads / 32 ? red[l] : -INFINITY;
-    s = l < kThreads / 32 ? red2[l] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      merge(m, s, m2, s2);
-    }
-    lse = (m + log2f(s)) * kLn2;
-    if (threadIdx.x == 0) {
-      a.loss[row] = top.any ? a.temp * a.temp * (top.kl + lse) : 0.f;
-      if (a.lse) a.lse[row] = lse;
-    }
-  } else {
-    lse = a.lse[row];
-  }
-  if (!GRAD) return;
-  T* dz = (T*)a.dz + row * a.lddz;
-  const float g = top.any ? (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * (a.inv_n ? *a.inv_n : 1.f) * a.temp : 0.f;
-  const float lse2 = lse * kLog2e;
-  float* total = smem + 3 * a.k;
-  dedup(top, a.k, total);
-  // 16-byte stores where the two rows lie alike
-  const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
-  for_row<T>(
-      z, a.V,
-      [&](int j, const Vec16<T>& v) {
-        Vec16<T> o;
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          o.v[e] = from_f32<T>(top.any ? g * ex2(fmaf(to_f32(v.v[e]), factor, -lse2)) : 0.f);
-        if (alike) {
-          *reinterpret_cast<Vec16<T>*>(dz + j) = o;
-        } else {
-#pragma unroll
-          for (int e = 0; e < N; ++e) dz[j + e] = o.v[e];
-        }
-      },
-      [&](int j, T v) { dz[j] = from_f32<T>(top.any ? g * ex2(fmaf(to_f32(v), factor, -lse2)) : 0.f); });
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.k; i += kThreads)
-    if (total[i] >= 0.f || total[i] != total[i])
-      dz[top.id[i]] = from_f32<T>(g * (ex2(fmaf(top.zk[i], factor, -lse2)) - total[i]));
-}
-
-// ------------------------------------------------------------------------------------------------------------
-constexpr int kHold = 256;            // threads of a holding CTA
-constexpr int kPiece = 8192;          // bytes of a bulk copy
-constexpr int kMaxHold = 96 * 1024;   // bytes of a row in one CTA at most
-constexpr int kHoldTarget = 64 * 1024;  // and as many as leave room for three CTAs an SM
-constexpr int kMaxCluster = 16;
+constexpr int kStream = 256;          // threads of a streaming CTA
 
 // Where a row's 16-byte vectors begin, and which of them a rank of `ranks` takes; single values at the ends belong
 // to the first and the last rank.
@@ -259,226 +76,67 @@ struct Slice {
   }
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-               "r"(bytes), "r"(bar)
-               : "memory");
+// 1 / max(sum of n, 1), by whole warps; 1 where n is null.
+__device__ __forceinline__ float inv_count(const int* n, int parts) {
+  if (!n) return 1.f;
+  int c = 0;
+  for (int i = threadIdx.x % 32; i < parts; i += 32) c += n[i];
+  return 1.f / (float)max(__reduce_add_sync(0xffffffffu, c), 1);
 }
-__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+
+// The larger of two words' values, each of 16 bits with the other's beside it, or of two f32.
+template <typename T>
+__device__ __forceinline__ uint32_t max_words(uint32_t a, uint32_t b) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+template <>
+__device__ __forceinline__ uint32_t max_words<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <>
+__device__ __forceinline__ uint32_t max_words<__half>(uint32_t a, uint32_t b) {
+  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kHold) distill_hold_kernel(DistillArgs a, int ranks) {
-  using W = Words<T>;
-  extern __shared__ __align__(16) uint8_t hold[];
-  __shared__ float red[32];
-  __shared__ float share[3][kMaxCluster];
-  __shared__ __align__(8) uint64_t bars[kMaxHold / kPiece];
-  __shared__ int abort_flag;
-  const int64_t row = blockIdx.x / ranks;
-  const int rank = blockIdx.x % ranks, tid = threadIdx.x;
-  const T* z = (const T*)a.z + row * a.ldz;
-  const Slice<T> sl(z, a.V, rank, ranks);
-  const int bytes = (sl.v1 - sl.v0) * 16, pieces = (bytes + kPiece - 1) / kPiece;
-  const uint32_t sbase = smem_u32(hold);
-  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (tid == 0) {
-    abort_flag = 0;
-    for (int i = 0; i < pieces; ++i) mbar_init(smem_u32(&bars[i]), 1);
-    fence_barrier_init();
-    for (int i = 0; i < pieces; ++i) {
-      const int n = min(kPiece, bytes - i * kPiece);
-      mbar_arrive_expect_tx(smem_u32(&bars[i]), n);
-      bulk_load(sbase + i * kPiece, reinterpret_cast<const uint8_t*>(z + sl.head) + (int64_t)sl.v0 * 16 + i * kPiece, n,
-                smem_u32(&bars[i]));
+// Entry i's total where it is the first with its id, else -1. ids is padded to whole fours with -1.
+__device__ __forceinline__ float first_total(const int* ids, const float* p, int k, int i) {
+  const int j = ids[i];
+  float total = 0.f;
+  for (int c = 0; c < k; c += 4) {
+    const int4 q = *reinterpret_cast<const int4*>(ids + c);
+    if (q.x == j || q.y == j || q.z == j || q.w == j) {
+      const int v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (v[e] == j) {
+          if (c + e < i) return -1.f;
+          total += p[c + e];
+        }
     }
   }
+  return total;
+}
 
-  // the teacher's entries: p of all of them; z and the loss's terms of those in this rank's part
-  const int held = (bytes + 15) & ~15;
-  float* p = reinterpret_cast<float*>(hold + held);
-  float* zk = p + a.k;
-  int* id = reinterpret_cast<int*>(p + 2 * a.k);
-  float top = -INFINITY;
-  bool nan = false;
-  for (int i = tid; i < a.k; i += kHold) {
-    const int64_t j = a.id[row * a.k + i];
-    const float t = a.t[row * a.k + i] * a.inv_t;
-    if (j >= a.V) set_status(BRAIN_ERR_BOUNDS, 711);
-    const bool on = j >= 0 && j < a.V && t != -INFINITY;
-    id[i] = on ? (int)j : -1;
-    p[i] = t;
-    if (on) {
-      top = fmaxf(top, t);
-      nan |= t != t;
-    }
-  }
-  const float factor = a.inv_t * kLog2e;
-  float m = -INFINITY, s = 0.f;
-  // the single values at the ends, one a thread
-  int end = -1;
-  if (rank == 0 && tid < sl.head) end = tid;
-  const int tail = sl.head + sl.nv * W::N;
-  if (rank == ranks - 1 && tid >= 32 && tid - 32 < a.V - tail) end = tail + tid - 32;
-  float zend = 0.f;
-  if (end >= 0) {
-    zend = to_f32(z[end]);
-    const float f = zend * factor;
-    merge(m, s, f, f == -INFINITY ? 0.f : ex2(f - f));
-  }
-  top = block_max_all(top, red);
-  const bool any = __syncthreads_or(top > -INFINITY || nan);  // (the barriers are set up, too)
-  float sum = 0.f;
-  for (int i = tid; i < a.k; i += kHold) {
-    p[i] = id[i] >= 0 ? expf(p[i] - top) : 0.f;
-    sum += p[i];
-  }
-  sum = block_sum_all(sum, red);
-
-  // ---- the running maximum and sum, over the pieces as they land
-  bool ok = true;
-  for (int c = 0; c < pieces; ++c) {
-    ok = ok && mbar_wait(smem_u32(&bars[c]), 0, BRAIN_ERR_TIMEOUT_FULL, 712, &abort_flag);
-    const int stop = min((c + 1) * kPiece, bytes);
-    constexpr int U = kPiece / (kHold * 16);
-    uint4 v[U];
-    float f[U][W::N], lm = -INFINITY;
+// Vector `v` to dz + j: in one store where dz lies on 16 bytes as z does.
+template <typename T>
+__device__ __forceinline__ void put(T* dz, int j, const uint4& v, bool alike) {
+  if (alike) {
+    __stcs(reinterpret_cast<uint4*>(dz + j), v);
+  } else {
+    const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = c * kPiece + (u * kHold + tid) * 16;
-      const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-      v[u] = at < stop ? *reinterpret_cast<const uint4*>(hold + at) : make_uint4(none, none, none, none);  // -inf
-#pragma unroll
-      for (int i = 0; i < 4; ++i) W::unpack(word(v[u], i), f[u] + i * W::PER);
-#pragma unroll
-      for (int e = 0; e < W::N; ++e) lm = fmaxf(lm, f[u][e]);
-    }
-    lm *= factor;
-    const float top2 = fmaxf(m, lm), base = top2 == -INFINITY ? 0.f : top2;
-    s *= m == -INFINITY ? 1.f : ex2(m - base);
-    m = top2;
-    float ls[2] = {};
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < W::N; ++e) ls[e & 1] += ex2(fmaf(f[u][e], factor, -base));
-    s += ls[0] + ls[1];
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    merge(m, s, m2, s2);
-  }
-  __shared__ float wm[kHold / 32], ws[kHold / 32];
-  if (tid % 32 == 0) {
-    wm[tid / 32] = m;
-    ws[tid / 32] = s;
-  }
-  float kl = 0.f;
-  for (int i = tid; i < a.k; i += kHold) {
-    const int j = id[i];
-    if (j < 0) continue;
-    const int v = j < sl.head || j >= tail ? -1 : (j - sl.head) / W::N;
-    const bool mine = j < sl.head ? rank == 0 : j >= tail ? rank == ranks - 1 : v >= sl.v0 && v < sl.v1;
-    const float pi = p[i] / sum;
-    p[i] = pi;
-    if (!mine) {
-      id[i] = -1 - j;  // another rank's
-      continue;
-    }
-    zk[i] = to_f32(v < 0 ? z[j] : reinterpret_cast<const T*>(hold)[j - sl.head - sl.v0 * W::N]);
-    if (pi != 0.f) kl += pi * (logf(pi) - zk[i] * a.inv_t);
-  }
-  kl = block_sum_all(kl, red);
-  if (ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all ranks run
-  if (tid < 32) {
-    m = tid < kHold / 32 ? wm[tid] : -INFINITY;
-    s = tid < kHold / 32 ? ws[tid] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      merge(m, s, m2, s2);
-    }
-    if (tid < ranks) {
-      const float out[3] = {m, s, kl};
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&share[i][rank]), tid)), "f"(out[i])
-                     : "memory");
-    }
-    __syncwarp();
-  }
-  if (ranks > 1)
-    cluster_sync();
-  else
-    __syncthreads();
-  m = share[0][0];
-  s = share[1][0];
-  kl = share[2][0];
-  for (int r = 1; r < ranks; ++r) {
-    merge(m, s, share[0][r], share[1][r]);
-    kl += share[2][r];
-  }
-  const float lse = (m + log2f(s)) * kLn2;
-  if (rank == 0 && tid == 0) {
-    a.loss[row] = any ? a.temp * a.temp * (kl + lse) : 0.f;
-    if (a.lse) a.lse[row] = lse;
-  }
-  if (!GRAD) return;
-
-  // ---- the gradient, in place
-  T* dz = (T*)a.dz + row * a.lddz;
-  const float g = any ? (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * (a.inv_n ? *a.inv_n : 1.f) * a.temp : 0.f;
-  const float lse2 = lse * kLog2e;
-  for (int at = tid * 16; at < bytes; at += kHold * 16) {
-    uint4 v = *reinterpret_cast<const uint4*>(hold + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[2];
-      W::unpack(word(v, i), f);
-#pragma unroll
-      for (int e = 0; e < W::PER; ++e) f[e] = any ? g * ex2(fmaf(f[e], factor, -lse2)) : 0.f;
-      set_word(v, i, W::pack(f));
-    }
-    *reinterpret_cast<uint4*>(hold + at) = v;
-  }
-  if (end >= 0) dz[end] = from_f32<T>(any ? g * ex2(fmaf(zend, factor, -lse2)) : 0.f);
-  __syncthreads();
-  // the first entry with an id takes the sum of all that share it, in their order
-  for (int i = tid; i < a.k; i += kHold) {
-    const int j = id[i];
-    if (j < 0) continue;
-    float total = 0.f;
-    bool first = true;
-    for (int c = 0; c < a.k; ++c)
-      if (id[c] == j) {
-        if (c < i) first = false;
-        total += p[c];
-      }
-    if (!first) continue;
-    const T d = from_f32<T>(g * (ex2(fmaf(zk[i], factor, -lse2)) - total));
-    if (j < sl.head || j >= tail)
-      dz[j] = d;
-    else
-      reinterpret_cast<T*>(hold)[j - sl.head - sl.v0 * W::N] = d;
-  }
-  fence_proxy_async();  // what was written here is read by the copies
-  __syncthreads();
-  if (tid == 0 && bytes > 0) {
-    uint8_t* to = reinterpret_cast<uint8_t*>(dz + sl.head) + (int64_t)sl.v0 * 16;
-    for (int i = 0; i < pieces; ++i) bulk_store(to + i * kPiece, sbase + i * kPiece, min(kPiece, bytes - i * kPiece));
-    tma_store_commit();
-    tma_store_wait_read<0>();  // the CTA's memory stays until it has been read
+    for (int i = 0; i < Words<T>::N; ++i) dz[j + i] = e[i];
   }
 }
 
 // The gradient from the kept log-sum-exp: a CTA a piece of a row, a vector of four a thread at a time.
 template <typename T>
-__global__ void __launch_bounds__(kHold) distill_grad_kernel(DistillArgs a, int ranks) {
+__global__ void __launch_bounds__(kStream) distill_grad_kernel(DistillArgs a, int ranks) {
   using W = Words<T>;
   constexpr int U = 4;
-  extern __shared__ float entries[];
+  extern __shared__ __align__(16) float entries[];
   __shared__ float red[32];
   const int64_t row = blockIdx.x / ranks;
   const int tid = threadIdx.x, rank = blockIdx.x % ranks;
@@ -486,26 +144,29 @@ __global__ void __launch_bounds__(kHold) distill_grad_kernel(DistillArgs a, int 
   T* dz = (T*)a.dz + row * a.lddz;
   const Slice<T> sl(z, a.V, rank, ranks);
   const uint4* zv = reinterpret_cast<const uint4*>(z + sl.head);
-  uint4* dv = reinterpret_cast<uint4*>(dz + sl.head);
+  const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
   // the first vectors are on their way while the entries are looked at
   uint4 v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (sl.v0 + u * kHold + tid < sl.v1) v[u] = zv[sl.v0 + u * kHold + tid];
-  float* p = entries;
+    if (sl.v0 + u * kStream + tid < sl.v1) v[u] = zv[sl.v0 + u * kStream + tid];
+  const int kp = (a.k + 3) & ~3;
+  int* id = reinterpret_cast<int*>(entries);
+  float* p = entries + kp;
   float* zk = p + a.k;
-  int* id = reinterpret_cast<int*>(p + 2 * a.k);
   float top = -INFINITY;
   bool nan = false;
   const int tail = sl.head + sl.nv * W::N;
-  for (int i = tid; i < a.k; i += kHold) {
+  for (int i = tid; i < kp; i += kStream) {
+    id[i] = -1;
+    if (i >= a.k) continue;
     const int64_t j = a.id[row * a.k + i];
     const float t = a.t[row * a.k + i] * a.inv_t;
     const bool on = j >= 0 && j < a.V && t != -INFINITY;
     const int at = (int)(on ? j : 0), w = (at - sl.head) / W::N;
     const bool mine = on && (at < sl.head ? rank == 0 : at >= tail ? rank == ranks - 1 : w >= sl.v0 && w < sl.v1);
-    id[i] = on ? (mine ? at : -1 - at) : INT32_MIN;
-    p[i] = t;
+    if (mine) id[i] = at;
+    p[i] = on ? t : -INFINITY;
     zk[i] = mine ? to_f32(z[at]) : 0.f;
     if (on) {
       top = fmaxf(top, t);
@@ -515,17 +176,18 @@ __global__ void __launch_bounds__(kHold) distill_grad_kernel(DistillArgs a, int 
   top = block_max_all(top, red);
   const bool any = __syncthreads_or(top > -INFINITY || nan);
   float sum = 0.f;
-  for (int i = tid; i < a.k; i += kHold) {
-    p[i] = id[i] != INT32_MIN ? expf(p[i] - top) : 0.f;
+  for (int i = tid; i < a.k; i += kStream) {
+    p[i] = p[i] == -INFINITY ? 0.f : expf(p[i] - top);
     sum += p[i];
   }
   sum = block_sum_all(sum, red);
   const float factor = a.inv_t * kLog2e, lse2 = a.lse[row] * kLog2e;
-  const float g = any ? (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * (a.inv_n ? *a.inv_n : 1.f) * a.temp : 0.f;
-  for (int at = sl.v0; at < sl.v1; at += U * kHold) {
+  const float by = inv_count(a.n, a.parts);
+  const float g = any ? (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * by * a.temp : 0.f;
+  for (int at = sl.v0; at < sl.v1; at += U * kStream) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = at + u * kHold + tid;
+      const int i = at + u * kStream + tid;
       if (i >= sl.v1) continue;
       uint4 o;
 #pragma unroll
@@ -536,127 +198,270 @@ __global__ void __launch_bounds__(kHold) distill_grad_kernel(DistillArgs a, int 
         for (int e = 0; e < W::PER; ++e) f[e] = any ? g * ex2(fmaf(f[e], factor, -lse2)) : 0.f;
         set_word(o, c, W::pack(f));
       }
-      dv[i] = o;
+      put(dz, sl.head + i * W::N, o, alike);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (at + (U + u) * kHold + tid < sl.v1) v[u] = zv[at + (U + u) * kHold + tid];
+      if (at + (U + u) * kStream + tid < sl.v1) v[u] = zv[at + (U + u) * kStream + tid];
   }
   int end = -1;
   if (rank == 0 && tid < sl.head) end = tid;
   if (rank == ranks - 1 && tid >= 32 && tid - 32 < a.V - tail) end = tail + tid - 32;
   if (end >= 0) dz[end] = from_f32<T>(any ? g * ex2(fmaf(to_f32(z[end]), factor, -lse2)) : 0.f);
   __syncthreads();
-  for (int i = tid; i < a.k; i += kHold) {
+  for (int i = tid; i < a.k; i += kStream) {
     const int j = id[i];
     if (j < 0) continue;
-    float total = 0.f;
-    bool first = true;
-    for (int c = 0; c < a.k; ++c)
-      if (id[c] == j) {
-        if (c < i) first = false;
-        total += p[c] / sum;
-      }
-    if (first) dz[j] = from_f32<T>(g * (ex2(fmaf(zk[i], factor, -lse2)) - total));
+    const float total = first_total(id, p, a.k, i);
+    if (!(total < 0.f)) dz[j] = from_f32<T>(g * (ex2(fmaf(zk[i], factor, -lse2)) - total / sum));
   }
 }
 
-// Rows that have an entry, counted before the gradient of a mean is written: a warp a row.
-__global__ void distill_count_kernel(const float* __restrict__ t, const int64_t* __restrict__ id, int64_t M, int k, int V,
-                                     int* __restrict__ count) {
-  const int lane = threadIdx.x % 32;
-  int n = 0;
-  for (int64_t row = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; row < M;
-       row += (int64_t)gridDim.x * (blockDim.x / 32)) {
-    bool any = false;
-    for (int i = lane; i - lane < k && !any; i += 32) {
-      const bool on = i < k && id[row * k + i] >= 0 && id[row * k + i] < V && t[row * k + i] != -INFINITY;
-      any = __any_sync(0xffffffffu, on);
+// Loss, or loss and gradient, a CTA a row: one pass for the maximum and sum, and for the gradient a second one,
+// which finds the row in L2.
+template <typename T, bool GRAD, int kRow, int U, int B>
+__global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
+  using W = Words<T>;
+  constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  extern __shared__ __align__(16) float entries[];
+  __shared__ float wm[kRow / 32], ws[kRow / 32], s_kl, s_sum;
+  __shared__ int s_any;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % 32;
+  const T* z = (const T*)a.z + row * a.ldz;
+  const Slice<T> sl(z, a.V, 0, 1);
+  const uint4* zv = reinterpret_cast<const uint4*>(z + sl.head);
+  const float factor = a.inv_t * kLog2e;
+  const int kp = (a.k + 3) & ~3, tail = sl.head + sl.nv * W::N;
+  int* id = reinterpret_cast<int*>(entries);
+  float* p = entries + kp;
+  float* zk = p + a.k;
+  float m = -INFINITY, s = 0.f;
+
+  uint4 v[U];
+  const auto load = [&](int at) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = at + u * kRow + tid;
+      v[u] = i < sl.nv ? __ldcg(zv + i) : make_uint4(kNone, kNone, kNone, kNone);
     }
-    n += any;
+  };
+  load(0);
+  for (int i = tid; i < kp; i += kRow) {
+    id[i] = -1;
+    if (i >= a.k) continue;
+    const int64_t j = a.id[row * a.k + i];
+    const float t = a.t[row * a.k + i] * a.inv_t;
+    if (j >= a.V) set_status(BRAIN_ERR_BOUNDS, 711);
+    const bool on = j >= 0 && j < a.V && t != -INFINITY;
+    if (on) id[i] = (int)j;
+    p[i] = on ? t : -INFINITY;
+    zk[i] = on ? to_f32(z[j]) : 0.f;
   }
-  if (lane == 0 && n) atomicAdd(count, n);
+  int end = -1;
+  if (tid < sl.head) end = tid;
+  if (tid >= 32 && tid - 32 < a.V - tail) end = tail + tid - 32;
+  float zend = 0.f;
+  if (end >= 0) {
+    zend = to_f32(z[end]);
+    const float f = zend * factor;
+    merge(m, s, f, f == -INFINITY ? 0.f : ex2(f - f));
+  }
+  for (int at = 0; at < sl.nv; at += U * kRow) {
+    uint32_t w[U * 4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u * 4] = v[u].x, w[u * 4 + 1] = v[u].y, w[u * 4 + 2] = v[u].z, w[u * 4 + 3] = v[u].w;
+    if (at + U * kRow < sl.nv) load(at + U * kRow);
+    uint32_t lw = w[0];
+#pragma unroll
+    for (int i = 1; i < U * 4; ++i) lw = max_words<T>(lw, w[i]);
+    float lm[2];
+    W::unpack(lw, lm);
+    if (W::PER == 2) lm[0] = fmaxf(lm[0], lm[1]);
+    const float top2 = fmaxf(m, lm[0] * factor), base = top2 == -INFINITY ? 0.f : top2;
+    s *= m == -INFINITY ? 1.f : ex2(m - base);
+    m = top2;
+    float ls[2] = {};
+#pragma unroll
+    for (int i = 0; i < U * 4; ++i) {
+      float f[2];
+      W::unpack(w[i], f);
+#pragma unroll
+      for (int e = 0; e < W::PER; ++e) ls[e] += ex2(fmaf(f[e], factor, -base));
+    }
+    s += ls[0] + ls[1];
+  }
+  if (GRAD) load(0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    merge(m, s, m2, s2);
+  }
+  if (lane == 0) {
+    wm[tid / 32] = m;
+    ws[tid / 32] = s;
+  }
+  __syncthreads();
+  if (tid < 32) {  // the teacher's softmax and the loss's own terms
+    float top = -INFINITY, sum = 0.f, kl = 0.f;
+    bool nan = false;
+    for (int i = lane; i < a.k; i += 32) {
+      top = fmaxf(top, p[i]);
+      nan |= p[i] != p[i];
+    }
+    top = warp_max(top);
+    const bool any = __any_sync(0xffffffffu, top > -INFINITY || nan);
+    for (int i = lane; i < a.k; i += 32) {
+      p[i] = p[i] == -INFINITY ? 0.f : expf(p[i] - top);
+      sum += p[i];
+    }
+    sum = warp_sum(sum);
+    for (int i = lane; i < a.k; i += 32) {
+      p[i] /= sum;
+      if (id[i] >= 0 && p[i] != 0.f) kl += p[i] * (logf(p[i]) - zk[i] * a.inv_t);
+    }
+    kl = warp_sum(kl);
+    if (lane == 0) {
+      s_any = any;
+      s_kl = kl;
+    }
+  }
+  m = lane < kRow / 32 ? wm[lane] : -INFINITY;
+  s = lane < kRow / 32 ? ws[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    merge(m, s, m2, s2);
+  }
+  const float lse = (m + log2f(s)) * kLn2;
+  __syncthreads();
+  const bool any = s_any;
+  if (tid == 0) {
+    a.loss[row] = any ? a.temp * a.temp * (s_kl + lse) : 0.f;
+    if (a.lse) a.lse[row] = lse;
+    if (a.counts) a.counts[row] = any;
+  }
+  if (!GRAD) return;
+
+  // ---- the gradient: g 2^x is 2^(x + log2 |g|), with its sign set afterwards
+  T* dz = (T*)a.dz + row * a.lddz;
+  const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
+  const float g = (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * inv_count(a.n, a.parts) * a.temp;
+  const float lse2 = lse * kLog2e, shift = log2f(fabsf(g)) - lse2;
+  const uint32_t sign = g < 0.f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
+  for (int at = 0; at < sl.nv; at += U * kRow) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = at + u * kRow + tid;
+      if (i >= sl.nv) continue;
+      uint4 o;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float f[2];
+        W::unpack(word(v[u], c), f);
+#pragma unroll
+        for (int e = 0; e < W::PER; ++e) f[e] = ex2(fmaf(f[e], factor, shift));
+        set_word(o, c, any ? W::pack(f) ^ sign : 0u);
+      }
+      put(dz, sl.head + i * W::N, o, alike);
+    }
+    if (at + U * kRow < sl.nv) load(at + U * kRow);
+  }
+  if (end >= 0) dz[end] = from_f32<T>(any ? g * ex2(fmaf(zend, factor, -lse2)) : 0.f);
+  __syncthreads();
+  if (any)
+    for (int i = tid; i < a.k; i += kRow) {
+      const int j = id[i];
+      if (j < 0) continue;
+      const float total = first_total(id, p, a.k, i);
+      if (!(total < 0.f)) dz[j] = from_f32<T>(g * (ex2(fmaf(zk[i], factor, -lse2)) - total));
+    }
 }
 
-// total = sum of the rows' losses (over the rows that count, with mean), inv_n = 1 / max(count, 1) or 1; one
-// block, so the sum has one order. loss or total may be null.
-__global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __restrict__ loss, int64_t M,
-                                                              const int* __restrict__ count, float* __restrict__ total,
-                                                              float* __restrict__ inv_n) {
+// n[block] = rows of the block's share that have an entry, before the gradient of a mean is written. Most rows have
+// their first entry, so a thread a row looks at one value.
+__global__ void __launch_bounds__(256) distill_count_kernel(const float* __restrict__ t, const int64_t* __restrict__ id,
+                                                            int64_t M, int k, int V, int* __restrict__ n) {
+  __shared__ int red[32];
+  int c = 0;
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < M; row += (int64_t)gridDim.x * 256) {
+    bool some = false;
+    for (int i = 0; i < k && !some; ++i) {
+      const int64_t j = id[row * k + i];
+      const float v = t[row * k + i];
+      some = j >= 0 && j < V && v != -INFINITY;
+    }
+    c += some;
+  }
+  c = block_sum_all(c, red);
+  if (threadIdx.x == 0) n[blockIdx.x] = c;
+}
+
+// total = sum of the rows' losses; where counts is given, divided by max(rows that count, 1), that number in *n (which
+// may be null); where it is not and n is, divided by max(sum of n, 1). One block, so the sum has one order.
+__global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __restrict__ loss,
+                                                              const float* __restrict__ counts, int64_t M, int* n,
+                                                              int parts, float* __restrict__ total) {
   __shared__ float red[32];
+  __shared__ int redi[32];
   float s = 0.f;
-  if (loss)
-    for (int64_t i = threadIdx.x; i < M; i += 1024) s += loss[i];
-  s = block_sum_all(s, red);
-  if (threadIdx.x == 0) {
-    const float inv = count ? 1.f / (float)max(*count, 1) : 1.f;
-    if (total) *total = s * inv;
-    if (inv_n) *inv_n = inv;
+  int c = 0;
+  for (int64_t i = threadIdx.x; i < M; i += 1024) {
+    s += loss[i];
+    if (counts) c += counts[i] != 0.f;
   }
-}
-
-template <typename T, bool GRAD>
-int launch_hold(const DistillArgs& a, int64_t M, int ranks, int held, cudaStream_t st) {
-  const auto kernel = distill_hold_kernel<T, GRAD>;
-  const int smem = held + a.k * 12;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxHold + 16 + kMaxTop * 12);
-  if (e == cudaSuccess && ranks > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return (int)e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(M * ranks));
-  cfg.blockDim = dim3(kHold);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = ranks;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, kernel, a, ranks);
+  s = block_sum_all(s, red);
+  float by = 1.f;
+  if (counts) {
+    c = block_sum_all(c, redi);
+    by = 1.f / (float)max(c, 1);
+    if (n && threadIdx.x == 0) *n = c;
+  } else {
+    by = inv_count(n, parts);
+  }
+  if (threadIdx.x == 0) *total = s * by;
 }
 
 template <typename T>
 int launch(const DistillArgs& a, int64_t M, cudaStream_t st) {
   const int64_t bytes = (int64_t)a.V * sizeof(T);
-  const bool alike = !a.dz || ((reinterpret_cast<uintptr_t>(a.z) ^ reinterpret_cast<uintptr_t>(a.dz)) & 15) == 0 &&
-                                  ((a.ldz - a.lddz) * sizeof(T)) % 16 == 0;
-  if (alike && !a.loss) {
+  const int smem = ((a.k + 3) & ~3) * 4 + a.k * 8;
+  if (!a.loss) {
     // pieces of 64 KB: short enough for an even end, long enough to hide the look at the entries
     const int ranks = (int)std::min<int64_t>((bytes + 65535) / 65536, INT32_MAX / M);
-    distill_grad_kernel<T><<<(unsigned)(M * ranks), kHold, a.k * 12, st>>>(a, ranks);
+    distill_grad_kernel<T><<<(unsigned)(M * ranks), kStream, smem, st>>>(a, ranks);
     return (int)cudaGetLastError();
   }
-  int ranks = 1;
-  while (ranks < kMaxCluster && bytes > ranks * (int64_t)kHoldTarget) ranks *= 2;
-  const int64_t held = ((bytes / 16 + ranks) / ranks) * 16;
-  if (alike && a.loss && held <= kMaxHold && M * ranks <= INT32_MAX)
-    return a.dz ? launch_hold<T, true>(a, M, ranks, (int)held, st) : launch_hold<T, false>(a, M, ranks, (int)held, st);
-  const size_t smem = (size_t)a.k * 16;
-  const unsigned grid = (unsigned)M;
-  if (a.loss && a.dz)
-    distill_kernel<T, true, true><<<grid, kThreads, smem, st>>>(a);
-  else if (a.loss)
-    distill_kernel<T, true, false><<<grid, kThreads, smem, st>>>(a);
-  else
-    distill_kernel<T, false, true><<<grid, kThreads, smem, st>>>(a);
-  return (int)cudaGetLastError();
+  const auto run = [&](auto grad, auto loss, int threads) {
+    if (a.dz)
+      grad<<<(unsigned)M, threads, smem, st>>>(a);
+    else
+      loss<<<(unsigned)M, threads, smem, st>>>(a);
+    return (int)cudaGetLastError();
+  };
+  // Short rows are bound by what a row costs besides its values, so many small CTAs share an SM; long ones, and few
+  // of them, by what one CTA has in flight (8192 x 4000 bf16: 74 us with 128 threads, 116 with 256, 218 with 512;
+  // 2048 x 50257: 125, 112, 130; 4096 x 128256: 547, 518, 503; the loss of 257 x 50257 f32: 30, 23, 20).
+  if (bytes > 131072 || M <= 2 * brain_host::num_sms())
+    return run(distill_row_kernel<T, true, 512, 4, 2>, distill_row_kernel<T, false, 512, 4, 2>, 512);
+  if (bytes > 16384) return run(distill_row_kernel<T, true, 256, 4, 4>, distill_row_kernel<T, false, 256, 4, 4>, 256);
+  return run(distill_row_kernel<T, true, 128, 4, 8>, distill_row_kernel<T, false, 128, 4, 8>, 128);
 }
 
 }  // namespace
 
 BRAIN_STATUS_READER(distill)
 
-// Rows: loss [M] (null: take lse), lse [M] (may be null with loss), dz (null: none; may be z) with its row
-// stride. The gradient is scaled by grad (null: 1; one a row with grad_rows) and inv_n (null: 1).
+// Rows: loss [M] (null: take lse), lse [M] (may be null with loss), counts [M] (may be null), dz (null: none; may
+// be z) with its row stride. The gradient is scaled by grad (null: 1; one a row with
+// grad_rows) and divided by the sum of n's parts (null: no division).
 BRAIN_API int brain_distill_rows(int dtype, const void* z, int64_t ldz, const float* t, const int64_t* id, float* loss,
-                                 float* lse, void* dz, int64_t lddz, const float* grad, const float* inv_n,
-                                 int grad_rows, int64_t M, int k, int V, float temp, cudaStream_t st) {
+                                 float* lse, float* counts, void* dz, int64_t lddz, const float* grad, const int* n,
+                                 int parts, int grad_rows, int64_t M, int k, int V, float temp, cudaStream_t st) {
   if (M <= 0) return 0;
   if (V <= 0 || k <= 0 || k > kMaxTop || M > INT32_MAX || !(temp > 0.f) || (!loss && (!dz || !lse)))
     return (int)cudaErrorInvalidValue;
-  const DistillArgs a{z, ldz, t, id, loss, lse, dz, lddz, grad, inv_n, grad_rows, k, V, 1.f / temp, temp};
+  const DistillArgs a{z, ldz, t, id, loss, lse, counts, dz, lddz, grad, n, parts, grad_rows, k, V, 1.f / temp, temp};
   switch (dtype) {
     case BRAIN_BF16: return launch<__nv_bfloat16>(a, M, st);
     case BRAIN_F16: return launch<__half>(a, M, st);
@@ -665,19 +470,16 @@ BRAIN_API int brain_distill_rows(int dtype, const void* z, int64_t ldz, const fl
   return (int)cudaErrorInvalidValue;
 }
 
-// count [1] (zeroed here) = rows with an entry.
-BRAIN_API int brain_distill_count(const float* t, const int64_t* id, int64_t M, int k, int V, int* count,
+// n [parts]: the rows with an entry, share by share.
+BRAIN_API int brain_distill_count(const float* t, const int64_t* id, int64_t M, int k, int V, int* n, int parts,
                                   cudaStream_t st) {
-  const cudaError_t e = cudaMemsetAsync(count, 0, sizeof(int), st);
-  if (e != cudaSuccess || M <= 0) return (int)e;
-  const int64_t blocks = (M + 7) / 8;
-  distill_count_kernel<<<(unsigned)(blocks < 1184 ? blocks : 1184), 256, 0, st>>>(t, id, M, k, V, count);
+  if (parts <= 0) return (int)cudaErrorInvalidValue;
+  distill_count_kernel<<<parts, 256, 0, st>>>(t, id, M, k, V, n);
   return (int)cudaGetLastError();
 }
 
-// total (null: not wanted) = sum of loss [M], over count with a mean (count not null); inv_n (null: not wanted).
-BRAIN_API int brain_distill_reduce(const float* loss, int64_t M, const int* count, float* total, float* inv_n,
+BRAIN_API int brain_distill_reduce(const float* loss, const float* counts, int64_t M, int* n, int parts, float* total,
                                    cudaStream_t st) {
-  distill_reduce_kernel<<<1, 1024, 0, st>>>(loss, M, count, total, inv_n);
+  distill_reduce_kernel<<<1, 1024, 0, st>>>(loss, counts, M, n, parts, total);
   return (int)cudaGetLastError();
 }

@@ -249,8 +249,14 @@ int plan_ranks(int64_t B, int V) {
 template <typename T>
 int launch(const VerifyArgs& a, int64_t B, cudaStream_t st) {
   const int ranks = plan_ranks(B, a.V);
-  cudaError_t e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return (int)e;
+  if (ranks > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return (int)e;
+  }
+  if (ranks == 1) {
+    verify_kernel<T><<<dim3(1, (unsigned)B), kThreads, 0, st>>>(a);
+    return (int)cudaGetLastError();
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ranks, (unsigned)B);
   cfg.blockDim = dim3(kThreads);

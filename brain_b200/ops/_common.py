@@ -49,9 +49,9 @@ _native.register({
     "brain_status_optim": ("brain_kernels", "pi"),
     "brain_status_attention": ("brain_kernels", "pi"),
     "brain_norm_fp8": ("brain_kernels", "iplplppppliifs"),
-    "brain_distill_rows": ("brain_kernels", "iplppppplppiliifs"),
-    "brain_distill_count": ("brain_kernels", "ppliips"),
-    "brain_distill_reduce": ("brain_kernels", "plppps"),
+    "brain_distill_rows": ("brain_kernels", "iplpppppplppiiliifs"),
+    "brain_distill_count": ("brain_kernels", "ppliipis"),
+    "brain_distill_reduce": ("brain_kernels", "pplpips"),
     "brain_status_distill": ("brain_kernels", "pi"),
     "brain_verify_draft": ("brain_kernels", "ipllpllpppppliis"),
     "brain_status_int4": ("brain_kernels", "pi"),
@@ -84,11 +84,17 @@ def dtype_code(name: str, t: torch.Tensor, allowed=(torch.bfloat16, torch.float1
 def launch(t: torch.Tensor, name: str, *args) -> None:
     """``_native.call`` with ``t``'s device current (a launch goes to the current device) and that device's
     current stream as the last argument."""
-    if t.device.index == torch.cuda.current_device():
-        _native.call(name, *args, _native.stream_ptr(t.device))
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        _native.call(name, *args, _raw_stream(index))
     else:
-        with torch.cuda.device(t.device):
-            _native.call(name, *args, _native.stream_ptr(t.device))
+        with torch.cuda.device(index):
+            _native.call(name, *args, _raw_stream(index))
+
+
+# the stream of a device as an integer, without the Stream object around it (2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: _native.stream_ptr(torch.device("cuda", index)))
 
 
 def no_backward(name: str, *tensors) -> None:
@@ -136,6 +142,8 @@ def main_grad_beta(p: torch.Tensor) -> float:
 
 def rows2d(x: torch.Tensor) -> torch.Tensor:
     """View x as [rows, last] with unit last-dim stride (copying only if needed)."""
+    if x.dim() == 2 and x.stride(1) == 1:
+        return x
     x2 = x.reshape(-1, x.shape[-1])
     if x2.stride(-1) != 1:
         x2 = x2.contiguous()

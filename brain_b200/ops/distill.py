@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._common import dtype_code, has_main_grad, launch, main_grad_beta, ptr, rows2d, same_device
+from ._common import DTYPE_CODES, dtype_code, has_main_grad, launch, main_grad_beta, ptr, rows2d, same_device
 from .gemm import gemm
 
 MAX_TOP = 1024
@@ -48,59 +48,68 @@ def _check(name, logits, teacher_logits, teacher_ids, temperature, reduction):
 
 
 def _teacher(teacher_logits, teacher_ids):
-    k = teacher_ids.shape[-1]
-    return (teacher_logits.detach().reshape(-1, k).float().contiguous(),
-            teacher_ids.reshape(-1, k).long().contiguous())
+    """The entries as contiguous float32 and int64 (their leading dimensions do not matter to the kernels)."""
+    t, ids = teacher_logits.detach(), teacher_ids
+    if t.dtype != torch.float32 or not t.is_contiguous():
+        t = t.float().contiguous()
+    if ids.dtype != torch.int64 or not ids.is_contiguous():
+        ids = ids.long().contiguous()
+    return t, ids
 
 
-def _rows(l2, t, ids, temperature, loss, lse, dz, grad=None, inv_n=None, grad_rows=False):
-    launch(l2, "brain_distill_rows", dtype_code("topk_distillation", l2), l2.data_ptr(), l2.stride(0), t.data_ptr(),
-           ids.data_ptr(), ptr(loss), ptr(lse), ptr(dz), 0 if dz is None else dz.stride(0), ptr(grad), ptr(inv_n),
-           int(grad_rows), l2.shape[0], t.shape[1], l2.shape[1], float(temperature))
+def _rows(l2, t, ids, temperature, loss, lse, counts, dz, grad=None, n=None, grad_rows=False):
+    launch(l2, "brain_distill_rows", DTYPE_CODES[l2.dtype], l2.data_ptr(), l2.stride(0), t.data_ptr(), ids.data_ptr(),
+           ptr(loss), ptr(lse), ptr(counts), ptr(dz), 0 if dz is None else dz.stride(0), ptr(grad), ptr(n),
+           0 if n is None else n.numel(), int(grad_rows), l2.shape[0], t.shape[-1], l2.shape[1], temperature)
 
 
-def _count(t, ids, V):
-    count = torch.empty(1, device=t.device, dtype=torch.int32)
-    launch(t, "brain_distill_count", t.data_ptr(), ids.data_ptr(), t.shape[0], t.shape[1], V, count.data_ptr())
-    return count
+def _count(t, ids, M, V):
+    """Numbers of the tokens that have an entry, in parts."""
+    n = t.new_empty(min(max(-(-M // 256), 1), 128), dtype=torch.int32)
+    launch(t, "brain_distill_count", t.data_ptr(), ids.data_ptr(), M, t.shape[-1], V, n.data_ptr(), n.numel())
+    return n
 
 
-def _reduce(loss, count, total, inv_n):
-    launch(count if loss is None else loss, "brain_distill_reduce", ptr(loss), 0 if loss is None else loss.numel(),
-           ptr(count), ptr(total), ptr(inv_n))
+def _total(loss, counts, n):
+    total = loss.new_empty(())
+    launch(loss, "brain_distill_reduce", loss.data_ptr(), ptr(counts), loss.shape[-1], ptr(n),
+           0 if n is None else n.numel(), total.data_ptr())
+    return total
 
 
-def _scalar(t):
-    return torch.empty((), device=t.device, dtype=torch.float32)
+def _loss(l2, t, ids, temperature, reduction, lse=None, n=None):
+    """The loss; where given, ``lse`` [M] and (of a mean) ``n`` [1] are written too."""
+    M = l2.shape[0]
+    if reduction != "mean":
+        loss = t.new_empty(M)
+        _rows(l2, t, ids, temperature, loss, lse, None, None)
+        return loss if reduction == "none" else _total(loss, None, None)
+    loss = t.new_empty((2, M))
+    _rows(l2, t, ids, temperature, loss, lse, loss[1], None)
+    return _total(loss, loss[1], n)
 
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, t, ids, temperature, reduction):
         l2 = rows2d(logits)
-        M, V = l2.shape
-        loss = torch.empty(M, device=logits.device, dtype=torch.float32)
-        lse = torch.empty_like(loss) if ctx.needs_input_grad[0] else None
-        _rows(l2, t, ids, temperature, loss, lse, None)
-        mean = reduction == "mean"
-        inv_n = _scalar(t) if mean and lse is not None else None
-        total = None
-        if reduction != "none":
-            total = _scalar(t)
-            _reduce(loss, _count(t, ids, V) if mean else None, total, inv_n)
-        ctx.save_for_backward(logits, t, ids, lse, inv_n)
+        lse = t.new_empty(l2.shape[0])
+        n = t.new_empty(1, dtype=torch.int32) if reduction == "mean" else None
+        loss = _loss(l2, t, ids, temperature, reduction, lse, n)
+        ctx.save_for_backward(logits, t, ids, lse, n)
         ctx.meta = temperature, reduction
-        return loss.view(logits.shape[:-1]) if total is None else total
+        return loss.view(logits.shape[:-1]) if reduction == "none" else loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        logits, t, ids, lse, inv_n = ctx.saved_tensors
+        logits, t, ids, lse, n = ctx.saved_tensors
         temperature, reduction = ctx.meta
         l2 = rows2d(logits)
-        out = torch.empty(l2.shape, device=logits.device, dtype=logits.dtype)
-        _rows(l2, t, ids, temperature, None, lse, out, g.reshape(-1).float().contiguous(), inv_n,
-              grad_rows=reduction == "none")
+        out = torch.empty_like(l2, memory_format=torch.contiguous_format)
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.float().contiguous()
+        _rows(l2, t, ids, temperature, None, lse, None, out, g, n, grad_rows=reduction == "none")
         return out.view(logits.shape), None, None, None, None
 
 
@@ -136,7 +145,10 @@ def topk_distillation(logits, teacher_logits, teacher_ids, temperature: float = 
         return topk_distillation_ref(logits, teacher_logits, teacher_ids, temperature, reduction)
     dtype_code("topk_distillation", logits)
     t, ids = _teacher(teacher_logits, teacher_ids)
-    return _DistillFn.apply(logits, t, ids, float(temperature), reduction)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _DistillFn.apply(logits, t, ids, float(temperature), reduction)
+    loss = _loss(rows2d(logits), t, ids, float(temperature), reduction)
+    return loss.view(logits.shape[:-1]) if reduction == "none" else loss
 
 
 def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: float = 1.0, reduction: str = "mean",
@@ -160,23 +172,13 @@ def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: flo
         t, ids = _teacher(teacher_logits, teacher_ids)
         l2 = rows2d(logits)
         if out is None:
-            out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        o2 = out.view(-1, out.shape[-1])
-        loss, total = _loss_and_grad(l2, t, ids, temperature, reduction, o2)
-        return loss.view(logits.shape[:-1]) if total is None else total, out
-
-
-def _loss_and_grad(l2, t, ids, temperature, reduction, out):
-    loss = torch.empty(l2.shape[0], device=l2.device, dtype=torch.float32)
-    count = inv_n = total = None
-    if reduction == "mean":
-        count, inv_n = _count(t, ids, l2.shape[1]), _scalar(t)
-        _reduce(None, count, None, inv_n)
-    _rows(l2, t, ids, temperature, loss, None, out, None, inv_n)
-    if reduction != "none":
-        total = _scalar(t)
-        _reduce(loss, count, total, None)
-    return loss, total
+            out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        o2 = out if out.dim() == 2 else out.view(-1, out.shape[-1])
+        M, V = l2.shape
+        n = _count(t, ids, M, V) if reduction == "mean" else None
+        loss = t.new_empty(M)
+        _rows(l2, t, ids, float(temperature), loss, None, None, o2, None, n)
+        return (loss.view(logits.shape[:-1]) if reduction == "none" else _total(loss, None, n)), out
 
 
 class _LinearDistillFn(torch.autograd.Function):
@@ -187,16 +189,16 @@ class _LinearDistillFn(torch.autograd.Function):
         chunk = min(chunk, M) if chunk else M
         dlogits = torch.empty(M, -(-V // 8) * 8, device=h.device, dtype=torch.bfloat16)[:, :V]  # 16-byte rows
         loss = torch.empty(M, device=h.device, dtype=torch.float32)
-        count, inv_n, total = _count(t, ids, V), _scalar(t), _scalar(t)
-        _reduce(None, count, None, inv_n)
+        k = t.shape[-1]
+        t, ids = t.view(M, k), ids.view(M, k)
+        n = _count(t, ids, M, V)
         for s0 in range(0, M, max(chunk, 1)):
             rows = slice(s0, min(M, s0 + chunk))
             gemm(h2[rows], w, trans_b=True, out=dlogits[rows])
-            _rows(dlogits[rows], t[rows], ids[rows], temperature, loss[rows], None, dlogits[rows], None, inv_n)
-        _reduce(loss, count, total, None)
+            _rows(dlogits[rows], t[rows], ids[rows], temperature, loss[rows], None, None, dlogits[rows], None, n)
         ctx.save_for_backward(h2, w, dlogits)
         ctx.hshape = h.shape
-        return total
+        return _total(loss, None, n)
 
     @staticmethod
     @once_differentiable

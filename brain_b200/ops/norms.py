@@ -191,10 +191,16 @@ def _norm_fp8(name, x, r, w, eps, scaling):
     x2 = rows2d(x)
     M = x2.shape[0]
     r2 = None if r is None else rows2d(r)
-    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     block = scaling == "block"
-    scale = torch.empty((*x.shape[:-1], D // 128) if block else x.shape[:-1], device=x.device, dtype=torch.float32)
-    s = None if r is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    scale = x.new_empty((M, D // 128) if block else M, dtype=torch.float32)
+    if x2 is x and x.stride(0) == D:  # as below, without the cost of shapes
+        q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+        s = None if r is None else torch.empty_like(x)
+    else:
+        q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+        s = None if r is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        if x.dim() != 2:
+            scale = scale.view(*x.shape[:-1], D // 128) if block else scale.view(x.shape[:-1])
     launch(x, "brain_norm_fp8", code, x2.data_ptr(), x2.stride(0), ptr(r2), 0 if r2 is None else r2.stride(0),
            w.contiguous().data_ptr(), ptr(s), q.data_ptr(), scale.data_ptr(), M, D, int(block), float(eps))
     return q, scale, s

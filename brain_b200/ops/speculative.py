@@ -47,14 +47,17 @@ def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_l
     q = draft_probs
     if q is not None and q.stride(2) != 1:
         q = q.contiguous()
-    drafted = draft_tokens.long().contiguous()
-    lens = None if draft_lens is None else draft_lens.int().contiguous()
+    drafted = draft_tokens if draft_tokens.dtype == torch.int64 else draft_tokens.long()
+    drafted = drafted.contiguous()
+    lens = draft_lens
+    if lens is not None:
+        lens = (lens if lens.dtype == torch.int32 else lens.int()).contiguous()
     u = uniforms.contiguous()
-    tokens = torch.empty(B, K1, device=p.device, dtype=torch.int64)
-    count = torch.empty(B, device=p.device, dtype=torch.int64)
-    launch(p, "brain_verify_draft", code, p.data_ptr(), p.stride(0), p.stride(1), ptr(q), 0 if q is None else q.stride(0),
-           0 if q is None else q.stride(1), drafted.data_ptr(), ptr(lens), u.data_ptr(), tokens.data_ptr(),
-           count.data_ptr(), B, K, V)
+    tokens = drafted.new_empty((B, K1))
+    count = drafted.new_empty(B)
+    ps, qs = p.stride(), (0, 0) if q is None else q.stride()
+    launch(p, "brain_verify_draft", code, p.data_ptr(), ps[0], ps[1], ptr(q), qs[0], qs[1], drafted.data_ptr(), ptr(lens),
+           u.data_ptr(), tokens.data_ptr(), count.data_ptr(), B, K, V)
     return tokens, count
 
 

@@ -99,14 +99,15 @@ def int4_linear(x, packed, scales, zeros=None, bias=None, group_size: int = 128)
     if packed.stride(1) != 1 or packed.stride(0) % 16 or packed.data_ptr() % 16:
         raise ValueError("int4_linear: the packed weight's rows have to be adjacent bytes that start on 16 bytes")
     x2 = rows2d(x)
+    M = x2.shape[0]
     if x2.stride(0) % 8 or x2.data_ptr() % 16:  # the kernel copies 16 bytes at a time
         x2 = x2.clone(memory_format=torch.contiguous_format)
-    y = torch.empty(*x.shape[:-1], N, device=x.device, dtype=x.dtype)
-    sums = torch.empty(x2.shape[0], N, device=x.device, dtype=torch.float32) if K > _SLAB else None
+    y = x.new_empty((M, N))
+    sums = x.new_empty((M, N), dtype=torch.float32) if K > _SLAB else None
     launch(x, "brain_int4_linear", code, x2.data_ptr(), x2.stride(0), packed.data_ptr(), packed.stride(0),
            scales.contiguous().data_ptr(), None if zeros is None else zeros.contiguous().data_ptr(), ptr(bias),
-           y.data_ptr(), ptr(sums), x2.shape[0], N, K, group_size)
-    return y
+           y.data_ptr(), ptr(sums), M, N, K, group_size)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
 class Int4Linear(torch.nn.Module):
