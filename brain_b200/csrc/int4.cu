@@ -33,7 +33,6 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTiles = 2;         // 32-row tiles between two meetings of the warps
 constexpr int kRound = 4;         // meetings of the warps between two of the cluster
 constexpr int kMaxCluster = 16;
 
@@ -52,23 +51,30 @@ struct Int4Args {
   uint32_t inv_g;
 };
 
-// c += A B: A 16 x 16, B 16 x 8
+// c = A B + (first ? 0 : c): A 16 x 16, B 16 x 8
+#define BRAIN_MMA(TYPES)                                                                                         \
+  if (first)                                                                                                     \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPES ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "    \
+                 "{%10,%10,%10,%10};"                                                                            \
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));                      \
+  else                                                                                                           \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPES ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "    \
+                 "{%0,%1,%2,%3};"                                                                                \
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 template <typename T>
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first);
 template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                                   bool first) {
+  BRAIN_MMA("bf16.bf16")
 }
 template <>
-__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  BRAIN_MMA("f16.f16")
 }
+#undef BRAIN_MMA
 
 // (w & mask) ^ flip in one operation
 __device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t flip) {
@@ -121,17 +127,19 @@ __device__ __forceinline__ uint32_t group_of(uint32_t k32, uint32_t inv_g) {
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-// for a warp that has written nothing that another CTA reads
+// where nothing has been written that another CTA reads
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// NT: 8-token tiles; KB: 32-wide K blocks a warp. A unit is 16 rows by 8 tokens.
-template <int NT, int KB>
+// NT: 8-token tiles; KB: 32-wide K blocks a warp; RT: 16-row halves a tile. A unit is 16 rows by 8 tokens.
+template <int NT, int KB, int RT>
 struct Layout {
   static constexpr int kStages = 2;                     // tiles in a warp's ring
-  static constexpr int kTile = 32 * KB * 16;            // bytes of a tile of a warp's K
+  static constexpr int kTiles = 4 / RT;                 // tiles between two meetings of the warps
+  static constexpr int kRows = 16 * RT;
+  static constexpr int kTile = kRows * KB * 16;            // bytes of a tile of a warp's K
   static constexpr int kRing = kWarps * kStages * kTile;
-  static constexpr int kUnits = kTiles * 2 * NT;
+  static constexpr int kUnits = kTiles * RT * NT;
   static constexpr int kPart = kUnits * kWarps * 512;   // [unit][warp][lane] float4
   static constexpr int places(int split) { return (kUnits * kRound + split - 1) / split; }
   static constexpr int recv(int split) { return split > 1 ? 2 * places(split) * split * 512 : 0; }
@@ -141,12 +149,13 @@ struct Layout {
 };
 
 // FL: groups that a scale may change at in 128 of K (128 / G, at least 1); ZP: zero points.
-template <typename T, int NT, int KB, int FL, bool ZP>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+template <typename T, int NT, int KB, int RT, int FL, bool ZP>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
     int4_kernel(const __grid_constant__ CUtensorMap wmap, const Int4Args a) {
-  using L = Layout<NT, KB>;
+  using L = Layout<NT, KB, RT>;
   constexpr int kGroups = KB / 4 * FL;  // sums taken apart in a warp's K
   constexpr int kGroupBlocks = KB / kGroups, kStages = L::kStages, kUnits = L::kUnits;
+  constexpr int kTiles = L::kTiles, kRows = L::kRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int split = gridDim.x, rank = blockIdx.x;
@@ -157,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
   const uint32_t bars = smem_u32(tail) + warp * kStages * 8, ring = smem_u32(smem) + warp * kStages * L::kTile;
 
-  const int tiles = (a.N + 31) / 32, m0 = blockIdx.z * 8 * NT;
+  const int tiles = (a.N + kRows - 1) / kRows, m0 = blockIdx.z * 8 * NT;
   const int t0 = (int)((int64_t)tiles * blockIdx.y / gridDim.y), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / gridDim.y);
   const int k0 = (rank * kWarps + warp) * KB * 32;
   const bool active = k0 < a.K;
@@ -165,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   if (threadIdx.x == 0) *abort_flag = 0;
   const auto fetch = [&](int t, int st) {
     mbar_arrive_expect_tx(bars + 8 * st, L::kTile);
-    tma_load_2d(&wmap, ring + st * L::kTile, bars + 8 * st, k0 / 2, t * 32);
+    tma_load_2d(&wmap, ring + st * L::kTile, bars + 8 * st, k0 / 2, t * kRows);
   };
   if (lane == 0) {
     for (int st = 0; st < kStages; ++st) mbar_init(bars + 8 * st, 1);
@@ -197,11 +206,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int q = 0; q < kGroups; ++q) {
         const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-        float c[4] = {};
+        float c[4];
 #pragma unroll
         for (int j = q * kGroupBlocks; j < (q + 1) * kGroupBlocks; ++j) {
-          mma<T>(c, ones, b[t][j][0], b[t][j][1]);
-          mma<T>(c, ones, b[t][j][2], b[t][j][3]);
+          mma<T>(c, ones, b[t][j][0], b[t][j][1], j == q * kGroupBlocks);
+          mma<T>(c, ones, b[t][j][2], b[t][j][3], false);
         }
         xsum[t][q][0] = c[0];
         xsum[t][q][1] = c[1];
@@ -209,21 +218,23 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   }
 
   // ---- scales and zero points of a tile's rows g, g + 8, .., asked for when the last tile is done
-  T sc[4][kGroups];
-  uint8_t zp[4][kGroups];
+  T sc[2 * RT][kGroups];
+  uint8_t zp[2 * RT][kGroups];
   uint32_t goff[kGroups];
 #pragma unroll
   for (int q = 0; q < kGroups; ++q)
     goff[q] = min(a.group0 + (int)group_of(k0 / 32 + q * kGroupBlocks, a.inv_g), a.groups - 1);
   const auto scales = [&](int t) {
-    const int64_t first = (int64_t)t * 32 * a.groups;
+    const T* sbase = (const T*)a.s + (int64_t)t * kRows * a.groups;
+    const uint8_t* zbase = ZP ? a.z + (int64_t)t * kRows * a.groups : nullptr;
+    const int last = a.N - 1 - t * kRows;  // rows past it repeat it, and are not stored
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const uint32_t row = min(h * 8 + g, a.N - 1 - t * 32) * a.groups;  // rows past the end are not stored
+    for (int h = 0; h < 2 * RT; ++h) {
+      const uint32_t row = min(h * 8 + g, last) * a.groups;
 #pragma unroll
       for (int q = 0; q < kGroups; ++q) {
-        sc[h][q] = ((const T*)a.s + first)[row + goff[q]];
-        if (ZP) zp[h][q] = (a.z + first)[row + goff[q]];
+        sc[h][q] = sbase[row + goff[q]];
+        if (ZP) zp[h][q] = zbase[row + goff[q]];
       }
     }
   };
@@ -232,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   // unit u of a round belongs to rank u % split, in place u / split
   const int places = L::places(split);
   const auto store = [&](int t, int u, float4 v) {  // unit u of the tile t: row half u / NT, tokens u % NT
-    const int n = t * 32 + u / NT * 16 + g, m = m0 + (u % NT) * 8 + t4 * 2;
+    const int n = t * kRows + u / NT * 16 + g, m = m0 + (u % NT) * 8 + t4 * 2;
     const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -250,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   };
   const auto finish = [&](int tr, int parity) {  // the owned units of the round that starts at tile tr
     for (int i = warp; i < places; i += kWarps) {
-      const int u = i * split + rank, t = tr + u / (2 * NT);
+      const int u = i * split + rank, t = tr + u / (RT * NT);
       if (u >= kUnits * kRound || t >= t1) continue;
       const float4* from = recv + ((parity * places + i) * split) * 32 + lane;
       float4 v = from[0];
@@ -258,33 +269,34 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         const float4 w = from[r * 32];
         v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
       }
-      store(t, u % (2 * NT), v);
+      store(t, u % (RT * NT), v);
     }
   };
 
   const Unpack<T, ZP> unpack;
   const uint8_t* wlane = smem + warp * kStages * L::kTile + g * (KB * 16) + t4 * 4;
   const uint32_t turn = (KB == 8 ? g : (g >> 1) & 3) * 16;  // the copy's swizzle of 16-byte blocks
-  int st = 0, parity = 0, meeting = 0;  // meeting: of the round
+  int st = 0, parity = 0, meeting = 0, turns = 0;  // meeting: of the round
+  const int inv_split = 65536 / split + 1;  // u inv_split >> 16 is u / split for the few units of a round
   uint32_t phase = 0;
   for (int tb = t0; tb < t1; tb += kTiles) {
     const bool closes = meeting == kRound - 1 || tb + kTiles >= t1;
-    if (tb > t0) asm volatile("bar.sync 1, 512;" ::: "memory");  // the last meeting's sums have been read
+    if (tb > t0) asm volatile("bar.sync 1, 384;" ::: "memory");  // the last meeting's sums have been read
 #pragma unroll 1
     for (int i = 0; i < kTiles; ++i) {
       const int t = tb + i;
-      float sum[2][NT][4] = {};
+      float sum[RT][NT][4] = {};
       if (active && t < t1) {
         mbar_wait(bars + 8 * st, phase, BRAIN_ERR_TIMEOUT_FULL, 801, abort_flag);
         const uint8_t* at = wlane + st * L::kTile;
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-          float acc[2][NT][4] = {};
+          float acc[RT][NT][4];
 #pragma unroll
           for (int j = q * kGroupBlocks; j < (q + 1) * kGroupBlocks; ++j) {
             const uint8_t* aj = at + (turn ^ (j * 16));
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RT; ++r) {
               uint32_t w[2][4];
 #pragma unroll
               for (int h = 0; h < 2; ++h)
@@ -292,13 +304,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
               const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma<T>(acc[r][n], a0, b[n][j][0], b[n][j][1]);
-                mma<T>(acc[r][n], a1, b[n][j][2], b[n][j][3]);
+                mma<T>(acc[r][n], a0, b[n][j][0], b[n][j][1], j == q * kGroupBlocks);
+                mma<T>(acc[r][n], a1, b[n][j][2], b[n][j][3], false);
               }
             }
           }
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
+          for (int h = 0; h < 2 * RT; ++h) {
             const float s = to_f32(sc[h][q]);
             const float off = ZP ? __int_as_float(0xcb000000u | zp[h][q]) + (8388608.f - 128.f) : -136.f;  // -128 - z
 #pragma unroll
@@ -318,45 +330,48 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         phase ^= st == 0;
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          part[(((i * 2 + r) * NT + n) * kWarps + warp) * 32 + lane] =
+          part[(((i * RT + r) * NT + n) * kWarps + warp) * 32 + lane] =
               make_float4(sum[r][n][0], sum[r][n][1], sum[r][n][2], sum[r][n][3]);
     }
-    __syncthreads();
+    // half of the warps, in turn, add up what all of them left; the others go on
+    const bool adds = (warp / (kWarps / 2)) == turns;
+    turns ^= 1;
     if (split > 1 && meeting == 0) {
       cluster_wait();  // at first: every CTA of the cluster runs; later: the last round's sums are here
       if (tb > t0) finish(tb - kTiles * kRound, parity ^ 1);
       __syncwarp();
     }
-    for (int u = warp; u < kUnits; u += kWarps) {
-      if (tb + u / (2 * NT) >= t1) continue;
-      const float4* from = part + u * kWarps * 32 + lane;
-      float4 v = from[0];
+    if (adds) {
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      for (int u = warp % (kWarps / 2); u < kUnits; u += kWarps / 2) {
+        if (tb + u / (RT * NT) >= t1) continue;
+        const float4* from = part + u * kWarps * 32 + lane;
+        float4 v = from[0];
 #pragma unroll
-      for (int k = 1; k < kWarps; ++k) {
-        const float4 w = from[k * 32];
-        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        for (int k = 1; k < kWarps; ++k) {
+          const float4 w = from[k * 32];
+          v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
+        if (split > 1) {
+          const int ur = meeting * kUnits + u, place = ur * inv_split >> 16, owner = ur - place * split;
+          const uint32_t to = mapa_shared(smem_u32(recv + ((parity * places + place) * split + rank) * 32 + lane), owner);
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                       : "memory");
+        } else {
+          store(tb + u / (RT * NT), u % (RT * NT), v);
+        }
       }
-      if (split > 1) {
-        const int ur = meeting * kUnits + u;
-        const uint32_t to =
-            mapa_shared(smem_u32(recv + ((parity * places + ur / split) * split + rank) * 32 + lane), ur % split);
-        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-                     : "memory");
-      } else {
-        store(tb + u / (2 * NT), u % (2 * NT), v);
-      }
+      __syncwarp();
+      if (tb + kTiles < t1) asm volatile("bar.arrive 1, 384;" ::: "memory");
+    } else {
+      asm volatile("bar.arrive 2, 256;" ::: "memory");
     }
-    __syncwarp();
-    if (tb + kTiles < t1) asm volatile("bar.arrive 1, 512;" ::: "memory");
     if (closes) {
       if (split > 1) {
-        if (warp < kUnits)
-          cluster_arrive();
-        else
-          cluster_arrive_relaxed();
+        cluster_arrive();
       }
       meeting = 0;
       parity ^= 1;
@@ -370,17 +385,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   }
 }
 
-template <typename T, int NT, int KB, int FL, bool ZP>
+template <typename T, int NT, int KB, int RT, int FL, bool ZP>
 int launch_tile(const Int4Args& a, const uint8_t* w, int64_t ldw, cudaStream_t st) {
-  using L = Layout<NT, KB>;
+  using L = Layout<NT, KB, RT>;
   CUtensorMap wmap;
   const uint64_t wd[2] = {(uint64_t)a.K / 2, (uint64_t)a.N}, ws[1] = {(uint64_t)ldw};
-  const uint32_t wb[2] = {KB * 16, 32};
+  const uint32_t wb[2] = {KB * 16, L::kRows};
   if (!brain_host::encode_tiled(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(w), wd, ws, wb,
                                 KB == 8 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
     return (int)cudaErrorInvalidValue;
-  const auto kernel = int4_kernel<T, NT, KB, FL, ZP>;
-  const int per = kWarps * KB * 32, split = (a.K + per - 1) / per, tiles = (a.N + 31) / 32;
+  const auto kernel = int4_kernel<T, NT, KB, RT, FL, ZP>;
+  const int per = kWarps * KB * 32, split = (a.K + per - 1) / per, tiles = (a.N + L::kRows - 1) / L::kRows;
   const int ntok = (a.M + 8 * NT - 1) / (8 * NT);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads);
@@ -416,8 +431,8 @@ int launch_tile(const Int4Args& a, const uint8_t* w, int64_t ldw, cudaStream_t s
 
 template <typename T, int FL, bool ZP>
 int launch_tokens(const Int4Args& a, const uint8_t* w, int64_t ldw, cudaStream_t st) {
-  if (a.M <= 8) return launch_tile<T, 1, 8, FL, ZP>(a, w, ldw, st);
-  return launch_tile<T, 2, 8, FL, ZP>(a, w, ldw, st);
+  if (a.M <= 8) return launch_tile<T, 1, 8, 2, FL, ZP>(a, w, ldw, st);
+  return launch_tile<T, 2, 8, 2, FL, ZP>(a, w, ldw, st);
 }
 
 template <typename T, bool ZP>
