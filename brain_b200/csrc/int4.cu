@@ -46,6 +46,7 @@ struct Int4Args {
   float* next;        // [M, N] where the sums go when more K follows, or null
   void* y;            // [M, N]
   int M, N, K, groups, group0;  // group0: the group that this K starts in
+  int vec;            // a warp's scales of a row, and zero points, are adjacent and start on their own size
   // k / G of a k that 32 divides is the high half of (k / 32) inv_g, inv_g the next whole number above
   // 2^32 / (G / 32): exact while (k / 32) (G / 32) < 2^32, and G <= K <= 2^20. 0: G is 32
   uint32_t inv_g;
@@ -217,9 +218,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
       }
   }
 
-  // ---- scales and zero points of a tile's rows g, g + 8, .., asked for when the last tile is done
-  T sc[2 * RT][kGroups];
-  uint8_t zp[2 * RT][kGroups];
+  // ---- scales and zero points of a tile's rows g, g + 8, .., asked for when the last tile is done: two scales and
+  // four zero points a register, brought in one load a row where they lie for that
+  constexpr int kScW = kGroups / 2, kZpW = (kGroups + 3) / 4;
+  uint32_t scw[2 * RT][kScW], zpw[2 * RT][kZpW];
+  const auto scale_at = [&](int h, int q) {
+    const uint32_t w = scw[h][q / 2];
+    float f[2];
+    Words<T>::unpack(w, f);
+    return f[q & 1];
+  };
+  const auto zero_at = [&](int h, int q) { return (int)(zpw[h][q / 4] >> (q % 4 * 8) & 255u); };
   uint32_t goff[kGroups];
 #pragma unroll
   for (int q = 0; q < kGroups; ++q)
@@ -231,10 +240,36 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
 #pragma unroll
     for (int h = 0; h < 2 * RT; ++h) {
       const uint32_t row = min(h * 8 + g, last) * a.groups;
+      if (a.vec) {
+        const T* sp = sbase + (row + goff[0]);
+        if (kGroups == 2) {
+          scw[h][0] = *reinterpret_cast<const uint32_t*>(sp);
+          if (ZP) zpw[h][0] = *reinterpret_cast<const uint16_t*>(zbase + (row + goff[0]));
+        } else if (kGroups == 4) {
+          const uint2 v = *reinterpret_cast<const uint2*>(sp);
+          scw[h][0] = v.x, scw[h][kScW / 2] = v.y;
+          if (ZP) zpw[h][0] = *reinterpret_cast<const uint32_t*>(zbase + (row + goff[0]));
+        } else {
+          const uint4 v = *reinterpret_cast<const uint4*>(sp);
 #pragma unroll
-      for (int q = 0; q < kGroups; ++q) {
-        sc[h][q] = sbase[row + goff[q]];
-        if (ZP) zp[h][q] = zbase[row + goff[q]];
+          for (int i = 0; i < kScW; ++i) scw[h][i] = word(v, i);
+          if (ZP) {
+            const uint2 z = *reinterpret_cast<const uint2*>(zbase + (row + goff[0]));
+            zpw[h][0] = z.x, zpw[h][kZpW - 1] = z.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kScW; ++i)
+          scw[h][i] = *reinterpret_cast<const uint16_t*>(sbase + (row + goff[2 * i])) |
+                      (uint32_t)*reinterpret_cast<const uint16_t*>(sbase + (row + goff[2 * i + 1])) << 16;
+        if (ZP)
+#pragma unroll
+          for (int i = 0; i < kZpW; ++i) {
+            zpw[h][i] = 0;
+#pragma unroll
+            for (int e = 0; e < 4 && i * 4 + e < kGroups; ++e) zpw[h][i] |= (uint32_t)zbase[row + goff[i * 4 + e]] << (e * 8);
+          }
       }
     }
   };
@@ -300,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
               uint32_t w[2][4];
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                unpack(*reinterpret_cast<const uint32_t*>(aj + (r * 2 + h) * 8 * (KB * 16)), ZP ? zp[r * 2 + h][q] : 8, w[h]);
+                unpack(*reinterpret_cast<const uint32_t*>(aj + (r * 2 + h) * 8 * (KB * 16)), ZP ? zero_at(r * 2 + h, q) : 8, w[h]);
               const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
@@ -311,8 +346,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
           }
 #pragma unroll
           for (int h = 0; h < 2 * RT; ++h) {
-            const float s = to_f32(sc[h][q]);
-            const float off = ZP ? __int_as_float(0xcb000000u | zp[h][q]) + (8388608.f - 128.f) : -136.f;  // -128 - z
+            const float s = scale_at(h, q);
+            const float off = ZP ? __int_as_float(0xcb000000u | zero_at(h, q)) + (8388608.f - 128.f) : -136.f;  // -128 - z
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -449,6 +484,9 @@ int launch(Int4Args a, int G, const uint8_t* w, int64_t ldw, float* sums, cudaSt
   constexpr int kSlab = kMaxCluster * 2048;
   const int K = a.K;
   const T* x = (const T*)a.x;
+  const int adjacent = 256 / G;  // groups in a warp's K
+  a.vec = (G == 32 || G == 64 || G == 128) && a.groups % adjacent == 0 && ((uintptr_t)a.s & (2 * adjacent - 1)) == 0 &&
+          ((uintptr_t)a.z & (adjacent - 1)) == 0;
   if (K > kSlab && (!sums || kSlab % G)) return (int)cudaErrorInvalidValue;
   for (int k = 0; k < K; k += kSlab) {
     a.x = x + k;
@@ -478,7 +516,7 @@ BRAIN_API int brain_int4_linear(int dtype, const void* x, int64_t ldx, const voi
   const int groups = (K + G - 1) / G;
   if (G > K) G = K;
   const uint32_t inv_g = G == 32 ? 0 : (uint32_t)((1ull << 32) / (G / 32)) + 1;
-  const Int4Args a{x, ldx, s, (const uint8_t*)z, bias, nullptr, nullptr, y, M, N, K, groups, 0, inv_g};
+  const Int4Args a{x, ldx, s, (const uint8_t*)z, bias, nullptr, nullptr, y, M, N, K, groups, 0, 0, inv_g};
   switch (dtype) {
     case BRAIN_BF16: return launch<__nv_bfloat16>(a, G, (const uint8_t*)w, ldw, sums, st);
     case BRAIN_F16: return launch<__half>(a, G, (const uint8_t*)w, ldw, sums, st);
