@@ -218,10 +218,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
       }
   }
 
-  // ---- scales and zero points of a tile's rows g, g + 8, .., asked for when the last tile is done: two scales and
+  // ---- scales and zero points of a tile's rows g, g + 8, .., asked for a tile ahead where registers allow: two scales and
   // four zero points a register, brought in one load a row where they lie for that
   constexpr int kScW = kGroups / 2, kZpW = (kGroups + 3) / 4;
-  uint32_t scw[2 * RT][kScW], zpw[2 * RT][kZpW];
+  constexpr bool kAhead = FL < 4;  // groups of 32 have too many
+  uint32_t scw[2 * RT][kScW], zpw[2 * RT][kZpW], sc_ahead[2 * RT][kScW], zp_ahead[2 * RT][kZpW];
+  auto& scn = kAhead ? sc_ahead : scw;
+  auto& zpn = kAhead ? zp_ahead : zpw;
   const auto scale_at = [&](int h, int q) {
     const uint32_t w = scw[h][q / 2];
     float f[2];
@@ -243,32 +246,32 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
       if (a.vec) {
         const T* sp = sbase + (row + goff[0]);
         if (kGroups == 2) {
-          scw[h][0] = *reinterpret_cast<const uint32_t*>(sp);
-          if (ZP) zpw[h][0] = *reinterpret_cast<const uint16_t*>(zbase + (row + goff[0]));
+          scn[h][0] = *reinterpret_cast<const uint32_t*>(sp);
+          if (ZP) zpn[h][0] = *reinterpret_cast<const uint16_t*>(zbase + (row + goff[0]));
         } else if (kGroups == 4) {
           const uint2 v = *reinterpret_cast<const uint2*>(sp);
-          scw[h][0] = v.x, scw[h][kScW / 2] = v.y;
-          if (ZP) zpw[h][0] = *reinterpret_cast<const uint32_t*>(zbase + (row + goff[0]));
+          scn[h][0] = v.x, scn[h][kScW / 2] = v.y;
+          if (ZP) zpn[h][0] = *reinterpret_cast<const uint32_t*>(zbase + (row + goff[0]));
         } else {
           const uint4 v = *reinterpret_cast<const uint4*>(sp);
 #pragma unroll
-          for (int i = 0; i < kScW; ++i) scw[h][i] = word(v, i);
+          for (int i = 0; i < kScW; ++i) scn[h][i] = word(v, i);
           if (ZP) {
             const uint2 z = *reinterpret_cast<const uint2*>(zbase + (row + goff[0]));
-            zpw[h][0] = z.x, zpw[h][kZpW - 1] = z.y;
+            zpn[h][0] = z.x, zpn[h][kZpW - 1] = z.y;
           }
         }
       } else {
 #pragma unroll
         for (int i = 0; i < kScW; ++i)
-          scw[h][i] = *reinterpret_cast<const uint16_t*>(sbase + (row + goff[2 * i])) |
+          scn[h][i] = *reinterpret_cast<const uint16_t*>(sbase + (row + goff[2 * i])) |
                       (uint32_t)*reinterpret_cast<const uint16_t*>(sbase + (row + goff[2 * i + 1])) << 16;
         if (ZP)
 #pragma unroll
           for (int i = 0; i < kZpW; ++i) {
-            zpw[h][i] = 0;
+            zpn[h][i] = 0;
 #pragma unroll
-            for (int e = 0; e < 4 && i * 4 + e < kGroups; ++e) zpw[h][i] |= (uint32_t)zbase[row + goff[i * 4 + e]] << (e * 8);
+            for (int e = 0; e < 4 && i * 4 + e < kGroups; ++e) zpn[h][i] |= (uint32_t)zbase[row + goff[i * 4 + e]] << (e * 8);
           }
       }
     }
@@ -325,6 +328,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
         mbar_wait(bars + 8 * st, phase, BRAIN_ERR_TIMEOUT_FULL, 801, abort_flag);
         const uint8_t* at = wlane + st * L::kTile;
 #pragma unroll
+        for (int h = 0; kAhead && h < 2 * RT; ++h) {
+#pragma unroll
+          for (int i = 0; i < kScW; ++i) scw[h][i] = scn[h][i];
+          if (ZP)
+#pragma unroll
+            for (int i = 0; i < kZpW; ++i) zpw[h][i] = zpn[h][i];
+        }
+        if (kAhead && t + 1 < t1) scales(t + 1);
+#pragma unroll
         for (int q = 0; q < kGroups; ++q) {
           float acc[RT][NT][4];
 #pragma unroll
@@ -360,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
         }
         __syncwarp();
         if (lane == 0 && t + kStages < t1) fetch(t + kStages, st);
-        if (t + 1 < t1) scales(t + 1);
+        if (!kAhead && t + 1 < t1) scales(t + 1);
         st = st == kStages - 1 ? 0 : st + 1;
         phase ^= st == 0;
       }
