@@ -12,9 +12,12 @@
 // their order, by the thread of the first, so the result is the same every time.
 //
 // Bound by memory: the logits once for the loss; once in and once out for the gradient. A CTA takes a row and, for
-// the gradient, reads it again right after the first pass, out of L2; the backward pass of autograd has the
-// log-sum-exp and streams pieces of rows. Exponentials are not what bounds: without them 2048 x 128256 takes 243 us
-// in place of 254.
+// the gradient, reads it again right after the first pass, out of L2 (or its own ring); the backward pass of autograd
+// has the log-sum-exp and streams pieces of rows. Measured on bf16 rows of 128256: loss of 2048 90 us (5.8 TB/s),
+// gradient alone 165 us (6.4), loss and gradient of 4096 466 us (4.5). Exponentials are not what bounds the last: it
+// took 243 us in place of 254 (for 2048, before the ring) without them. Holding a row on chip for both passes, with a
+// cluster of CTAs, was slower: 560 us with CTAs that load, exchange their sums and store in turn, and 1300 us as a
+// persistent pipeline, whose exchange and entries cost each row several microseconds in a row.
 #include <algorithm>
 #include <type_traits>
 
@@ -218,13 +221,24 @@ __global__ void __launch_bounds__(kStream) distill_grad_kernel(DistillArgs a, in
 }
 
 // Loss, or loss and gradient, a CTA a row: one pass for the maximum and sum, and for the gradient a second one,
-// which finds the row in L2.
-template <typename T, bool GRAD, int kRow, int U, int B>
+// which finds the row in L2. Every thread has a ring of its own in shared memory, filled by asynchronous copies S
+// blocks (of U vectors a thread) ahead: while one CTA of an SM writes, the other has to read at the whole rate, which
+// takes about 64 KB on their way. The last S blocks of the first pass are still there for the second.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <typename T, bool GRAD, int kRow, int U, int S, int B>
 __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
   using W = Words<T>;
   constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
   extern __shared__ __align__(16) float entries[];
-  __shared__ float wm[kRow / 32], ws[kRow / 32], s_kl, s_sum;
+  __shared__ float wm[kRow / 32], ws[kRow / 32], s_kl;
   __shared__ int s_any;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % 32;
@@ -233,20 +247,27 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
   const uint4* zv = reinterpret_cast<const uint4*>(z + sl.head);
   const float factor = a.inv_t * kLog2e;
   const int kp = (a.k + 3) & ~3, tail = sl.head + sl.nv * W::N;
-  int* id = reinterpret_cast<int*>(entries);
-  float* p = entries + kp;
+  // the ring, then the entries
+  uint4* ring = reinterpret_cast<uint4*>(entries) + tid;
+  int* id = reinterpret_cast<int*>(entries) + S * U * kRow * 4;
+  float* p = reinterpret_cast<float*>(id) + kp;
   float* zk = p + a.k;
   float m = -INFINITY, s = 0.f;
+  const float by = GRAD ? inv_count(a.n, a.parts) : 0.f;
 
-  uint4 v[U];
-  const auto load = [&](int at) {
+  const int blocks = (sl.nv + U * kRow - 1) / (U * kRow);
+  const auto load = [&](int block, int slot) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = at + u * kRow + tid;
-      v[u] = i < sl.nv ? __ldcg(zv + i) : make_uint4(kNone, kNone, kNone, kNone);
+      const int i = (block * U + u) * kRow + tid;
+      if (i < sl.nv) copy16(smem_u32(ring + (slot * U + u) * kRow), zv + i);
     }
   };
-  load(0);
+#pragma unroll
+  for (int c = 0; c < S; ++c) {
+    if (c < blocks) load(c, c);
+    copy_commit();
+  }
   for (int i = tid; i < kp; i += kRow) {
     id[i] = -1;
     if (i >= a.k) continue;
@@ -267,11 +288,16 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
     const float f = zend * factor;
     merge(m, s, f, f == -INFINITY ? 0.f : ex2(f - f));
   }
-  for (int at = 0; at < sl.nv; at += U * kRow) {
+  int slot = 0;
+  for (int block = 0; block < blocks; ++block) {
+    copy_wait<S - 1>();
     uint32_t w[U * 4];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u * 4] = v[u].x, w[u * 4 + 1] = v[u].y, w[u * 4 + 2] = v[u].z, w[u * 4 + 3] = v[u].w;
-    if (at + U * kRow < sl.nv) load(at + U * kRow);
+    for (int u = 0; u < U; ++u) {
+      uint4 v = ring[(slot * U + u) * kRow];
+      if ((block * U + u) * kRow + tid >= sl.nv) v = make_uint4(kNone, kNone, kNone, kNone);
+      w[u * 4] = v.x, w[u * 4 + 1] = v.y, w[u * 4 + 2] = v.z, w[u * 4 + 3] = v.w;
+    }
     uint32_t lw = w[0];
 #pragma unroll
     for (int i = 1; i < U * 4; ++i) lw = max_words<T>(lw, w[i]);
@@ -290,8 +316,10 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
       for (int e = 0; e < W::PER; ++e) ls[e] += ex2(fmaf(f[e], factor, -base));
     }
     s += ls[0] + ls[1];
+    if (block + S < blocks) load(block + S, slot);
+    copy_commit();
+    slot = slot == S - 1 ? 0 : slot + 1;
   }
-  if (GRAD) load(0);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
@@ -346,26 +374,34 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
   // ---- the gradient: g 2^x is 2^(x + log2 |g|), with its sign set afterwards
   T* dz = (T*)a.dz + row * a.lddz;
   const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
-  const float g = (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * inv_count(a.n, a.parts) * a.temp;
+  const float g = (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * by * a.temp;
   const float lse2 = lse * kLog2e, shift = log2f(fabsf(g)) - lse2;
   const uint32_t sign = g < 0.f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
-  for (int at = 0; at < sl.nv; at += U * kRow) {
+  // what the ring holds first (its oldest block is in `slot`), then the others from the row's start
+  const int kept = min(S, blocks);
+  if (blocks < S) slot = 0;
+  for (int c = 0; c < blocks; ++c) {
+    const int block = c < kept ? blocks - kept + c : c - kept;
+    copy_wait<S - 1>();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = at + u * kRow + tid;
+      const int i = (block * U + u) * kRow + tid;
       if (i >= sl.nv) continue;
+      const uint4 v = ring[(slot * U + u) * kRow];
       uint4 o;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int e4 = 0; e4 < 4; ++e4) {
         float f[2];
-        W::unpack(word(v[u], c), f);
+        W::unpack(word(v, e4), f);
 #pragma unroll
         for (int e = 0; e < W::PER; ++e) f[e] = ex2(fmaf(f[e], factor, shift));
-        set_word(o, c, any ? W::pack(f) ^ sign : 0u);
+        set_word(o, e4, any ? W::pack(f) ^ sign : 0u);
       }
       put(dz, sl.head + i * W::N, o, alike);
     }
-    if (at + U * kRow < sl.nv) load(at + U * kRow);
+    if (c + kept < blocks) load(c, slot);  // the (c + kept)-th in this order
+    copy_commit();
+    slot = slot == S - 1 ? 0 : slot + 1;
   }
   if (end >= 0) dz[end] = from_f32<T>(any ? g * ex2(fmaf(zend, factor, -lse2)) : 0.f);
   __syncthreads();
@@ -432,20 +468,22 @@ int launch(const DistillArgs& a, int64_t M, cudaStream_t st) {
     distill_grad_kernel<T><<<(unsigned)(M * ranks), kStream, smem, st>>>(a, ranks);
     return (int)cudaGetLastError();
   }
-  const auto run = [&](auto grad, auto loss, int threads) {
-    if (a.dz)
-      grad<<<(unsigned)M, threads, smem, st>>>(a);
-    else
-      loss<<<(unsigned)M, threads, smem, st>>>(a);
+  const auto run = [&](auto kernel, int threads, int ring) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring + smem);
+    if (e != cudaSuccess) return (int)e;
+    kernel<<<(unsigned)M, threads, ring + smem, st>>>(a);
     return (int)cudaGetLastError();
   };
   // Short rows are bound by what a row costs besides its values, so many small CTAs share an SM; long ones, and few
-  // of them, by what one CTA has in flight (8192 x 4000 bf16: 74 us with 128 threads, 116 with 256, 218 with 512;
-  // 2048 x 50257: 125, 112, 130; 4096 x 128256: 547, 518, 503; the loss of 257 x 50257 f32: 30, 23, 20).
-  if (bytes > 131072 || M <= 2 * brain_host::num_sms())
-    return run(distill_row_kernel<T, true, 512, 4, 2>, distill_row_kernel<T, false, 512, 4, 2>, 512);
-  if (bytes > 16384) return run(distill_row_kernel<T, true, 256, 4, 4>, distill_row_kernel<T, false, 256, 4, 4>, 256);
-  return run(distill_row_kernel<T, true, 128, 4, 8>, distill_row_kernel<T, false, 128, 4, 8>, 128);
+  // of them, by what one CTA has in flight (8192 x 4000 bf16: 79 us with 128 threads, 128 with 256, 232 with 512;
+  // 2048 x 50257: 115, 109, 134; 4096 x 128256: 575, 535, 466).
+  const auto pick = [&](auto grad) {
+    constexpr bool kGrad = decltype(grad)::value;
+    if (bytes > 131072 || M <= brain_host::num_sms()) return run(distill_row_kernel<T, kGrad, 512, 4, 3, 2>, 512, 512 * 4 * 3 * 16);
+    if (bytes > 16384) return run(distill_row_kernel<T, kGrad, 256, 4, 3, 4>, 256, 256 * 4 * 3 * 16);
+    return run(distill_row_kernel<T, kGrad, 128, 4, 3, 8>, 128, 128 * 4 * 3 * 16);
+  };
+  return a.dz ? pick(std::true_type()) : pick(std::false_type());
 }
 
 }  // namespace
