@@ -151,6 +151,22 @@ def topk_distillation(logits, teacher_logits, teacher_ids, temperature: float = 
     return loss.view(logits.shape[:-1]) if reduction == "none" else loss
 
 
+def _apart(out, logits):
+    """Whether every element of ``out`` is its own, and none is another element of ``logits``."""
+    span = 1
+    for size, stride in sorted(zip(out.shape, out.stride()), key=lambda x: x[1]):
+        if size > 1 and stride < span:
+            return False
+        span += (size - 1) * stride
+    if out.numel() == 0 or out.untyped_storage().data_ptr() != logits.untyped_storage().data_ptr() \
+            or (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()):
+        return True
+    size = out.element_size()
+    other = 1 + sum((n - 1) * s for n, s in zip(logits.shape, logits.stride()))
+    lo, lo2 = out.data_ptr(), logits.data_ptr()
+    return lo + span * size <= lo2 or lo2 + other * size <= lo
+
+
 def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: float = 1.0, reduction: str = "mean",
                            out: torch.Tensor | None = None):
     """(loss, dloss/dlogits) of :func:`topk_distillation` (with ``"none"`` the gradient of the losses' sum),
@@ -161,6 +177,8 @@ def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: flo
     if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.stride(-1) != 1):
         raise ValueError(f"{name}: out {tuple(out.shape)} {out.dtype} for logits {tuple(logits.shape)} {logits.dtype}")
     same_device(logits, out)
+    if out is not None and not _apart(out, logits):
+        raise ValueError(f"{name}: out shares memory with itself or with logits without being logits")
     if not logits.is_cuda:
         with torch.enable_grad():
             z = logits.detach().requires_grad_()

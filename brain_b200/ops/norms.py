@@ -191,6 +191,7 @@ def _norm_fp8(name, x, r, w, eps, scaling):
     x2 = rows2d(x)
     M = x2.shape[0]
     r2 = None if r is None else rows2d(r)
+    w = w.contiguous()
     block = scaling == "block"
     scale = x.new_empty((M, D // 128) if block else M, dtype=torch.float32)
     if x2 is x and x.stride(0) == D:  # as below, without the cost of shapes
@@ -202,7 +203,7 @@ def _norm_fp8(name, x, r, w, eps, scaling):
         if x.dim() != 2:
             scale = scale.view(*x.shape[:-1], D // 128) if block else scale.view(x.shape[:-1])
     launch(x, "brain_norm_fp8", code, x2.data_ptr(), x2.stride(0), ptr(r2), 0 if r2 is None else r2.stride(0),
-           w.contiguous().data_ptr(), ptr(s), q.data_ptr(), scale.data_ptr(), M, D, int(block), float(eps))
+           w.data_ptr(), ptr(s), q.data_ptr(), scale.data_ptr(), M, D, int(block), float(eps))
     return q, scale, s
 
 

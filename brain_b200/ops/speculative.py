@@ -11,7 +11,7 @@ from ._common import dtype_code, launch, ptr, same_device
 def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_lens=None):
     """Which drafted tokens the target's probabilities accept -> (tokens [B, K + 1], accepted [B]), int64.
 
-    ``target_probs`` [B, K + 1, V]: the target's probabilities after the context and each drafted token;
+    ``target_probs`` [B, K + 1, V] (up to 65535 sequences): the target's probabilities after the context and each drafted token;
     ``draft_tokens`` [B, K]; ``draft_probs`` [B, K, V]: what each token was drawn from (None: the draft was
     certain of its tokens); ``draft_lens`` [B]: how many of the K were drafted (None: all); ``uniforms``
     [B, K + 1] in [0, 1): one number a drafted token, the last for the token that follows.
@@ -51,7 +51,7 @@ def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_l
     drafted = drafted.contiguous()
     lens = draft_lens
     if lens is not None:
-        lens = (lens if lens.dtype == torch.int32 else lens.int()).contiguous()
+        lens = (lens if lens.dtype == torch.int32 else lens.clamp(0, K).int()).contiguous()
     u = uniforms.contiguous()
     tokens = drafted.new_empty((B, K1))
     count = drafted.new_empty(B)

@@ -80,8 +80,9 @@ def dequantize_int4(packed, scales, zeros=None, group_size: int = 128) -> torch.
 
 def int4_linear(x, packed, scales, zeros=None, bias=None, group_size: int = 128) -> torch.Tensor:
     """y = x @ W^T (+ bias) for x [..., K] bf16 or f16 and a packed 4-bit W (:func:`quantize_int4`); scales and
-    bias are of x's type. Values, products and sums are exact or f32 up to the rounding of y. The weight's rows
-    have to start on 16 bytes. Inference only."""
+    bias are of x's type. Values are exact, products and sums f32, and y is rounded once; a bf16 token with an
+    infinite entry (or one above 2^120) gives NaN. The weight is read once for every 16 tokens (8 of up to 8): for
+    few of them. Its rows have to start on 16 bytes. Inference only."""
     N, K = _check_weight(packed, scales, zeros, group_size)
     if x.dim() == 0 or x.shape[-1] != K:
         raise ValueError(f"int4_linear: x {tuple(x.shape)} for a weight [{N}, {K}]")
@@ -102,11 +103,13 @@ def int4_linear(x, packed, scales, zeros=None, bias=None, group_size: int = 128)
     M = x2.shape[0]
     if x2.stride(0) % 8 or x2.data_ptr() % 16:  # the kernel copies 16 bytes at a time
         x2 = x2.clone(memory_format=torch.contiguous_format)
+    # held until the launch: a copy let go of earlier could be given to the next one
+    scales, zeros = scales.contiguous(), None if zeros is None else zeros.contiguous()
+    bias = None if bias is None else bias.contiguous()
     y = x.new_empty((M, N))
     sums = x.new_empty((M, N), dtype=torch.float32) if K > _SLAB else None
     launch(x, "brain_int4_linear", code, x2.data_ptr(), x2.stride(0), packed.data_ptr(), packed.stride(0),
-           scales.contiguous().data_ptr(), None if zeros is None else zeros.contiguous().data_ptr(), ptr(bias),
-           y.data_ptr(), ptr(sums), M, N, K, group_size)
+           scales.data_ptr(), ptr(zeros), ptr(bias), y.data_ptr(), ptr(sums), M, N, K, group_size)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 

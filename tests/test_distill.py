@@ -131,6 +131,14 @@ def test_refusals():
         ops.topk_distillation(z, t.clone().requires_grad_(), ids)
     with pytest.raises(ValueError):
         ops.topk_distillation_grad(z, t, ids, out=torch.empty(3, 21))
+    both = torch.zeros(7, 20)
+    both[:3] = z
+    for out in (both[1:4], torch.empty(1, 20).expand(3, 20), both[:3].t().reshape(3, 20).t().t()[:, :0]):
+        with pytest.raises(ValueError):
+            ops.topk_distillation_grad(both[:3], t, ids, out=out)
+    want = ops.topk_distillation_grad(z, t, ids)[1]
+    assert torch.equal(ops.topk_distillation_grad(both[:3], t, ids, out=both[3:6])[1], want)
+    assert torch.equal(ops.topk_distillation_grad(both[:3], t, ids, out=both[:3])[1], want)
     with pytest.raises(ValueError):
         ops.linear_topk_distillation(torch.randn(3, 8), torch.randn(20, 9), t, ids)
 

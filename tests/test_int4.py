@@ -123,6 +123,12 @@ def test_strided_inputs_and_shapes(M):
     check(y, xs, w, None, torch.bfloat16)
     y = Q.int4_linear(x.cuda().transpose(0, 1)[..., 3:387], packed.cuda(), scales.t().contiguous().cuda().t(), z.cuda())
     check(y, xs.transpose(0, 1), w, None, torch.bfloat16)
+    # copies of both, each of the other's size, and zero points outside 0 .. 15
+    g = torch.Generator().manual_seed(9)
+    z = torch.randint(0, 256, (50, 3), generator=g, dtype=torch.uint8)
+    y = Q.int4_linear(x.cuda()[..., 3:387], packed.cuda(), scales.t().contiguous().cuda().t(),
+                      z.t().contiguous().cuda().t())
+    check(y, xs, dense(packed, scales, z, 128), None, torch.bfloat16)
     for off in (1, 8):
         with pytest.raises(ValueError):
             Q.int4_linear(x.cuda()[..., 3:387], big[:, off:off + 192], scales.cuda(), z.cuda())

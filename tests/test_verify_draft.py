@@ -130,7 +130,7 @@ def test_strides_and_index_types():
     bq = torch.zeros(3, 4, 500)
     bq[:] = q.transpose(0, 1)
     got = ops.verify_draft(big.cuda()[:, 1:5, 3:503], x.int().cuda(), u.t().contiguous().cuda().t(), bq.cuda().transpose(0, 1),
-                           torch.full((4,), 3).cuda())
+                           torch.full((4,), 2 ** 32 + 3).cuda())
     same(got, want)
     turned = p.transpose(1, 2).contiguous().cuda().transpose(1, 2)
     same(ops.verify_draft(turned, x.cuda(), u.cuda(), q.cuda()), want)
