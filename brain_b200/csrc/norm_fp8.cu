@@ -7,7 +7,8 @@
 // and q. The floor of the scale keeps its reciprocal finite for rows of subnormal size.
 //
 // Bound by memory: 7 bytes an element at 16 bits (x, r in; s, q out) against about 12 operations. A row stays in
-// registers between its two reductions, so it is read once. The first kernel for this took 37 instructions an
+// registers between its two reductions, so it is read once: 8192 rows of 4096 bf16 values with a residual take 38.2 us,
+// 6.1 TB/s, 94 % of what a copy reaches. The first kernel for this took 37 instructions an
 // element and kept the issue slots 77 % busy; so values are converted in pairs, s w is held in f32 after the
 // sum of squares, and rstd enters once a row, in the maximum and in the factor rstd / scale.
 #include "elem.cuh"
@@ -87,7 +88,7 @@ __device__ __forceinline__ uint32_t four_e4m3(float a, float b, float c, float d
 }
 
 // Rows of whole, aligned 16-byte vectors, VPT of them a thread. WARP: a warp a row, eight rows a CTA, no block
-// barrier (up to 128 vectors a row); else a CTA a row.
+// barrier (up to 64 vectors a row); else a CTA a row.
 template <typename T, int VPT, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : VPT == 4 ? 1024 : 512)
     norm_fp8_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ res, int64_t ldres,
@@ -208,10 +209,12 @@ int launch(const void* x, int64_t ldx, const void* res, int64_t ldres, const voi
                                                         (uint8_t*)q, scales, D, block, eps);
     return (int)cudaGetLastError();
   }
+  // Measured on 33.5 million bf16 values with a residual: 256 wide, a warp a row 39.6 us and a CTA 70.1; 512 wide, 36.5
+  // and 39.2; 1024 wide, 37.3 and 37.0. 8192 wide, two vectors a thread 39.4 us and four 38.3; a quarter of the rows,
+  // 13.1 and 13.8, as more threads wait at once where the last CTAs weigh more.
   if (nvec <= 32) return run(norm_fp8_kernel<T, 1, true>, 8, 256);
   if (nvec <= 64) return run(norm_fp8_kernel<T, 2, true>, 8, 256);
-  if (nvec <= 128) return run(norm_fp8_kernel<T, 4, true>, 8, 256);
-  if (nvec <= 512) return run(norm_fp8_kernel<T, 2, false>, 1, threads(2));
+  if (nvec <= 512 || (nvec <= 1024 && M <= 16 * brain_host::num_sms())) return run(norm_fp8_kernel<T, 2, false>, 1, threads(2));
   return run(norm_fp8_kernel<T, 4, false>, 1, threads(4));
 }
 
