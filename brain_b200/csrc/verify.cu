@@ -13,8 +13,13 @@
 //
 // Bound by memory: one row of p a sequence and one of q where a token is refused; the rows of the other
 // positions are touched at one value each. A cluster of CTAs shares a row, as many as fill the GPU at this
-// batch; each warp sums one contiguous segment, with 16-byte loads where the rows lie alike, and only the
+// batch; each warp sums one contiguous segment, with 16-byte loads where the rows start on 16 bytes, and only the
 // segment that holds the border is read again, out of cache. p alone is summed only where p - q is empty.
+// 256 sequences of 128256 f32 ids with draft probabilities take 52 us (5.0 TB/s), 32 take 11, one of 32000 ids 6.1.
+// Reading a CTA's share from front to back, all warps together, took 50, 13 and 7.2: the sums of its sections then
+// have to be put together out of those of all threads.
+#include <type_traits>
+
 #include "elem.cuh"
 
 using namespace brain;
@@ -23,7 +28,7 @@ namespace {
 
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = 8;
 
 struct VerifyArgs {
   const void *p, *q;            // target [B, K + 1, V], draft [B, K, V] or null
@@ -36,7 +41,14 @@ struct VerifyArgs {
   int K, V;
 };
 
-__device__ __forceinline__ float weight(float v) { return v > 0.f && v < INFINITY ? v : 0.f; }
+// v, but NaN where it is infinite, as v * 0 is; a maximum then passes over it as over any NaN.
+__device__ __forceinline__ float finite(float v) { return fmaf(v, 0.f, v); }
+__device__ __forceinline__ float weight(float v) { return fmaxf(finite(v), 0.f); }
+// max(weight(a) - weight(b), 0)
+__device__ __forceinline__ double excess(float a, float b) {
+  const float w = weight(b);
+  return (double)fmaxf(finite(a), w) - (double)w;
+}
 
 // Weights of one distribution over the vocabulary: p less q, p without the id `hole`, or p.
 template <typename T>
@@ -44,8 +56,7 @@ struct Mass {
   const T *p, *q;
   int hole;
   __device__ __forceinline__ double operator()(int j) const {
-    const float a = weight(to_f32(p[j])), b = q ? weight(to_f32(q[j])) : 0.f;
-    return a > b && j != hole ? (double)a - (double)b : 0.0;
+    return j != hole ? excess(to_f32(p[j]), q ? to_f32(q[j]) : 0.f) : 0.0;
   }
 };
 
@@ -62,35 +73,42 @@ __device__ __forceinline__ double segment_rows(const T* p, const T* q, int from,
   constexpr int U = 4;
   const int lane = threadIdx.x % 32;
   double s = 0;
-  const auto add = [&](float pj, float qj) {
-    const float a = weight(pj);
-    if (Q) {
-      const float b = weight(qj);
-      if (a > b) s += (double)a - (double)b;
-    } else {
-      s += (double)a;
-    }
-  };
+  const auto add = [&](float pj, float qj) { s += Q ? excess(pj, qj) : (double)weight(pj); };
   int j = from;
-  if (vec)
-    for (; j + U * 32 * W::N <= to; j += U * 32 * W::N) {
-      uint4 a[U], b[U];
+  const auto block = [&](auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;
+    const T *pj = p + j + lane * W::N, *qj = q + j + lane * W::N;
+    const int left = (to - j) / W::N - lane;
+    uint4 a[U], b[U];
 #pragma unroll
-      for (int c = 0; c < U; ++c) a[c] = *reinterpret_cast<const uint4*>(p + j + (c * 32 + lane) * W::N);
-      if (Q)
-#pragma unroll
-        for (int c = 0; c < U; ++c) b[c] = *reinterpret_cast<const uint4*>(q + j + (c * 32 + lane) * W::N);
-#pragma unroll
-      for (int c = 0; c < U; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float f[2], g[2] = {0.f, 0.f};
-          W::unpack(word(a[c], i), f);
-          if (Q) W::unpack(word(b[c], i), g);
-#pragma unroll
-          for (int e = 0; e < W::PER; ++e) add(f[e], g[e]);
-        }
+    for (int c = 0; c < U; ++c) {
+      if (!kWhole) a[c] = make_uint4(0, 0, 0, 0);
+      if (kWhole || c * 32 < left) a[c] = *reinterpret_cast<const uint4*>(pj + c * 32 * W::N);
     }
+    if (Q)
+#pragma unroll
+      for (int c = 0; c < U; ++c) {
+        if (!kWhole) b[c] = make_uint4(0, 0, 0, 0);
+        if (kWhole || c * 32 < left) b[c] = *reinterpret_cast<const uint4*>(qj + c * 32 * W::N);
+      }
+#pragma unroll
+    for (int c = 0; c < U; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float f[2], g[2] = {0.f, 0.f};
+        W::unpack(word(a[c], i), f);
+        if (Q) W::unpack(word(b[c], i), g);
+#pragma unroll
+        for (int e = 0; e < W::PER; ++e) add(f[e], g[e]);
+      }
+  };
+  if (vec) {
+    for (; j + U * 32 * W::N <= to; j += U * 32 * W::N) block(std::true_type());
+    if (j + W::N <= to) {
+      block(std::false_type());
+      j += (to - j) / W::N * W::N;
+    }
+  }
   for (j += lane; j + 15 * 32 < to; j += 16 * 32) {
     T a[16], b[16];
 #pragma unroll
@@ -239,20 +257,19 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(VerifyArgs a) {
   if (threadIdx.x == 0) a.count[b] = n;
 }
 
-// CTAs a sequence: as many as run at once (two an SM), no more than leave a warp 128 ids.
+// CTAs a sequence: as many as run at once (two an SM), no more than leave a warp 256 ids. Measured on f32 rows of 128256
+// ids with draft probabilities, 1, 2, 4, 8 CTAs: 8 sequences 19.6, 12.5, 9.3, 7.5 us; 32: 25.5, 16.3, 11.9, 11.0; 64:
+// 27.5, 18.8, 17.2, 22.7; 128: 31.2, 27.3, 31.1, 38.6; 256: 51.1, 53.3, 56.4, 71.1. Sixteen were slower at all of them. One
+// sequence of 32000: 8.4, 6.9, 6.1, 6.4.
 int plan_ranks(int64_t B, int V) {
   int c = 1;
-  while (c < kMaxCluster && B * c * 2 <= 2 * brain_host::num_sms() && V / (c * 2 * kWarps) >= 128) c *= 2;
+  while (c < kMaxCluster && B * c * 2 <= 2 * brain_host::num_sms() && V / (c * 2 * kWarps) >= 256) c *= 2;
   return c;
 }
 
 template <typename T>
 int launch(const VerifyArgs& a, int64_t B, cudaStream_t st) {
   const int ranks = plan_ranks(B, a.V);
-  if (ranks > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return (int)e;
-  }
   if (ranks == 1) {
     verify_kernel<T><<<dim3(1, (unsigned)B), kThreads, 0, st>>>(a);
     return (int)cudaGetLastError();
