@@ -1,4 +1,4 @@
-// Element types of the kernels that take bf16, f16 or f32 alike: conversions, 16-byte vectors, block sums.
+// Element types of the kernels that take bf16, f16 or f32 alike: conversions, words of 16-byte vectors, block sums.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -27,13 +27,6 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
-
-// 16 bytes of T, kept packed until used.
-template <typename T>
-struct alignas(16) Vec16 {
-  static constexpr int N = 16 / sizeof(T);
-  T v[N];
-};
 
 // 16 bytes as four 32-bit words, and the values of a word: two of 16 bits, or one f32.
 template <typename T>
@@ -92,13 +85,6 @@ __device__ __forceinline__ float block_max_all(float v, float* red) {
   if (l == 0) red[w] = v;
   __syncthreads();
   return warp_max(l < nw ? red[l] : -INFINITY);
-}
-
-// A value in another rank's shared memory (address from mapa_shared).
-__device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
 }
 
 }  // namespace brain

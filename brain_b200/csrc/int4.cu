@@ -6,16 +6,20 @@
 // in the way is unpacking: at the memory's rate an SM has about 40 cycles for 1 KB of weights (2048 values), and
 // its logic pipe does 64 operations a cycle. The tensor cores' warp-level 16 x 8 x 16 product takes 16 output
 // rows of the weight as its rows and 8 tokens as its columns. Its order along K is free as long as both sides
-// agree, so a lane takes the pairs (i, i + 4) that a shift and a mask leave in the two halves of a word of eight
-// values, and pairs the activations alike.
-//   bf16: a nibble masked onto the exponent bits of 128 is 128 + v exactly, and stays so: the group's sum less
-//     (128 + offset) times the group's sum of x, which a product with ones gives once. That costs the f32 sum of
-//     128 products up to 8 roundings at 34 times the size of its terms, 8e-6 of sum |x w|, against 2^-9 of y.
-//   f16: on the exponent bits of 1024 the same would cost eight times that, near f16's own step. There the
-//     offset comes off each pair, exactly: 1024 + v less 1024 + offset for a low nibble, and for a high one,
-//     which stands for 1024 + 16 v where it is, a 16th of that less 64 + offset, with no shift.
-// (Operands of 8 bits were slower: e4m3, which holds 0 .. 15, is taken apart into 16-bit products on this chip,
-// and whole numbers need three digits of each token and their sums put together.)
+// agree, so a lane takes the pairs (i, i + 4) that a mask leaves in the two halves of a word of eight values, and pairs
+// the activations alike.
+// A nibble masked onto the exponent bits of 1024 is the f16 value 1024 + v, and 1024 + offset comes off each pair,
+// exactly; a high nibble stands for 1024 + 16 v where it is, so a 16th of that less 64 + offset needs no shift. bf16
+// tokens are multiplied as f16 too, by a power of two that brings the largest of a token's values in a warp's K to
+// [2^14, 2^15): a bf16 value has fewer bits than f16's, so all above 2^-28 of the largest are exact, and the others off by
+// at most 2^-39 of it, far below the sum's own f32. (bf16 operands, whose 7 bits need three shifts a word and leave the
+// offset to be taken off the sums, took 65.0 us where this takes 60.2, at 8 x 57344 x 8192, groups of 64; 33.4 and 33.8
+// at 4 x 28672 x 8192; 5.6 and 6.1 at 1 x 4096 x 4096. They turned large tokens into NaN.)
+//
+// Measured: 1 x 4096 x 4096 6.1 us; 4 x 28672 x 8192 with zero points, groups of 128, 33.8 us (3.6 TB/s, 56 % of what a
+// copy reaches); 7 x 128256 x 4096, groups of 64, 62.7 us (4.5 TB/s, 68 %); 16 x 28672 x 8192 49.5 us; 32 tokens 87 us.
+// (Operands of 8 bits were slower at 4 x 28672 x 8192, 57 and 41 us: e4m3, which holds 0 .. 15, is taken apart into
+// 16-bit products on this chip, and whole numbers need three digits of each token and their sums put together.)
 //
 // A warp owns 256 of K for the whole call and keeps its tokens' operand registers; it streams tiles of 32 rows
 // of its K through a ring of TMA copies of its own, with no barrier to other warps. Eight warps make a CTA, a
@@ -35,6 +39,12 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRound = 4;         // meetings of the warps between two of the cluster
 constexpr int kMaxCluster = 16;
+constexpr int kBlocks = 8;        // 32-wide blocks of K a warp
+constexpr int kHalves = 2;        // 16-row halves of a tile
+constexpr int kRows = 16 * kHalves;
+constexpr int kTile = kRows * kBlocks * 16;  // bytes of a tile of a warp's K
+constexpr int kStages = 2;        // tiles in a warp's ring
+constexpr int kTiles = 2;         // tiles between two meetings of the warps
 
 struct Int4Args {
   const void* x;      // [M, K]
@@ -53,29 +63,16 @@ struct Int4Args {
 };
 
 // c = A B + (first ? 0 : c): A 16 x 16, B 16 x 8
-#define BRAIN_MMA(TYPES)                                                                                         \
-  if (first)                                                                                                     \
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPES ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "    \
-                 "{%10,%10,%10,%10};"                                                                            \
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                \
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));                      \
-  else                                                                                                           \
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPES ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "    \
-                 "{%0,%1,%2,%3};"                                                                                \
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                \
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  if (first)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-template <typename T>
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first);
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
-                                                   bool first) {
-  BRAIN_MMA("bf16.bf16")
 }
-template <>
-__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
-  BRAIN_MMA("f16.f16")
-}
-#undef BRAIN_MMA
 
 // (w & mask) ^ flip in one operation
 __device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t flip) {
@@ -84,24 +81,10 @@ __device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t fli
   return v;
 }
 
-// The four pairs (i, i + 4) of a word: as 128 + v for bf16, less their offset for f16. Two's complement values
-// have their top bit flipped, which makes them an offset of 8. The constants are held in registers.
-template <typename T, bool ZP>
-struct Unpack;
+// The four pairs (i, i + 4) of a word, less their offset. Two's complement values have their top bit flipped, which
+// makes them an offset of 8. The constants are held in registers.
 template <bool ZP>
-struct Unpack<__nv_bfloat16, ZP> {
-  uint32_t mask, flip;
-  __device__ __forceinline__ Unpack() {
-    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
-    asm volatile("mov.b32 %0, %1;" : "=r"(flip) : "n"(ZP ? 0x43004300 : 0x43084308));
-  }
-  __device__ __forceinline__ void operator()(uint32_t w, int, uint32_t (&q)[4]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = pick(w >> (4 * i), mask, flip);
-  }
-};
-template <bool ZP>
-struct Unpack<__half, ZP> {
+struct Unpack {
   uint32_t mask, flip, high_mask, high_flip;
   __device__ __forceinline__ Unpack() {
     asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
@@ -132,15 +115,11 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// NT: 8-token tiles; KB: 32-wide K blocks a warp; RT: 16-row halves a tile. A unit is 16 rows by 8 tokens.
-template <int NT, int KB, int RT>
+// NT: 8-token tiles. A unit is 16 rows by 8 tokens.
+template <int NT>
 struct Layout {
-  static constexpr int kStages = 2;                     // tiles in a warp's ring
-  static constexpr int kTiles = 4 / RT;                 // tiles between two meetings of the warps
-  static constexpr int kRows = 16 * RT;
-  static constexpr int kTile = kRows * KB * 16;            // bytes of a tile of a warp's K
   static constexpr int kRing = kWarps * kStages * kTile;
-  static constexpr int kUnits = kTiles * RT * NT;
+  static constexpr int kUnits = kTiles * kHalves * NT;
   static constexpr int kPart = kUnits * kWarps * 512;   // [unit][warp][lane] float4
   static constexpr int places(int split) { return (kUnits * kRound + split - 1) / split; }
   static constexpr int recv(int split) { return split > 1 ? 2 * places(split) * split * 512 : 0; }
@@ -150,13 +129,12 @@ struct Layout {
 };
 
 // FL: groups that a scale may change at in 128 of K (128 / G, at least 1); ZP: zero points.
-template <typename T, int NT, int KB, int RT, int FL, bool ZP>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
+template <typename T, int NT, int FL, bool ZP>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     int4_kernel(const __grid_constant__ CUtensorMap wmap, const Int4Args a) {
-  using L = Layout<NT, KB, RT>;
-  constexpr int kGroups = KB / 4 * FL;  // sums taken apart in a warp's K
-  constexpr int kGroupBlocks = KB / kGroups, kStages = L::kStages, kUnits = L::kUnits;
-  constexpr int kTiles = L::kTiles, kRows = L::kRows;
+  using L = Layout<NT>;
+  constexpr int kGroups = kBlocks / 4 * FL;  // sums taken apart in a warp's K
+  constexpr int kGroupBlocks = kBlocks / kGroups, kUnits = L::kUnits;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int split = gridDim.x, rank = blockIdx.x;
@@ -165,17 +143,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
   uint8_t* tail = smem + L::kRing + L::kPart + L::recv(split);
   int* abort_flag = reinterpret_cast<int*>(tail + kWarps * kStages * 8);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
-  const uint32_t bars = smem_u32(tail) + warp * kStages * 8, ring = smem_u32(smem) + warp * kStages * L::kTile;
+  const uint32_t bars = smem_u32(tail) + warp * kStages * 8, ring = smem_u32(smem) + warp * kStages * kTile;
 
   const int tiles = (a.N + kRows - 1) / kRows, m0 = blockIdx.z * 8 * NT;
   const int t0 = (int)((int64_t)tiles * blockIdx.y / gridDim.y), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / gridDim.y);
-  const int k0 = (rank * kWarps + warp) * KB * 32;
+  const int k0 = (rank * kWarps + warp) * kBlocks * 32;
   const bool active = k0 < a.K;
 
   if (threadIdx.x == 0) *abort_flag = 0;
   const auto fetch = [&](int t, int st) {
-    mbar_arrive_expect_tx(bars + 8 * st, L::kTile);
-    tma_load_2d(&wmap, ring + st * L::kTile, bars + 8 * st, k0 / 2, t * kRows);
+    mbar_arrive_expect_tx(bars + 8 * st, kTile);
+    tma_load_2d(&wmap, ring + st * kTile, bars + 8 * st, k0 / 2, t * kRows);
   };
   if (lane == 0) {
     for (int st = 0; st < kStages; ++st) mbar_init(bars + 8 * st, 1);
@@ -186,43 +164,54 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
   __syncthreads();
   if (split > 1) cluster_arrive_relaxed();
 
-  // ---- this warp's tokens: the pairs of token t * 8 + g, and (bf16) the groups' sums of tokens t4 * 2, + 1
-  constexpr bool kSums = std::is_same<T, __nv_bfloat16>::value;
-  uint32_t b[NT][KB][4];
-  float xsum[NT][kGroups][2];
+  // ---- this warp's tokens: the pairs of token t * 8 + g, and (bf16) what undoes the factor of tokens t4 * 2, + 1
+  constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
+  uint32_t b[NT][kBlocks][4];
+  float undo[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int m = m0 + t * 8 + g;
     const uint8_t* row = (const uint8_t*)a.x + (m * a.ldx + k0 + t4 * 8) * 2;
+    uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < KB; ++j) {
+    for (int j = 0; j < kBlocks; ++j) {
       uint4 v = make_uint4(0, 0, 0, 0);
       if (m < a.M && k0 + j * 32 < a.K) v = *reinterpret_cast<const uint4*>(row + j * 64);
       b[t][j][0] = __byte_perm(v.x, v.z, 0x5410);
       b[t][j][1] = __byte_perm(v.x, v.z, 0x7632);
       b[t][j][2] = __byte_perm(v.y, v.w, 0x5410);
       b[t][j][3] = __byte_perm(v.y, v.w, 0x7632);
+      // the bits of an absolute value rise with it
+      if (kScaled)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = __vmaxu2(top, b[t][j][i] & 0x7fff7fffu);
     }
-    if (kSums)
+    if (kScaled) {
+      top = max(top & 0xffffu, top >> 16);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^(14 - e) and its inverse, both normal, for a largest value in [2^e, 2^(e + 1)): e + 127 is top >> 7
+      const int e = max((int)(top >> 7), 15);
+      const float factor = __int_as_float((268 - e) << 23), inverse = __int_as_float((e - 14) << 23);
 #pragma unroll
-      for (int q = 0; q < kGroups; ++q) {
-        const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-        float c[4];
+      for (int j = 0; j < kBlocks; ++j)
 #pragma unroll
-        for (int j = q * kGroupBlocks; j < (q + 1) * kGroupBlocks; ++j) {
-          mma<T>(c, ones, b[t][j][0], b[t][j][1], j == q * kGroupBlocks);
-          mma<T>(c, ones, b[t][j][2], b[t][j][3], false);
+        for (int i = 0; i < 4; ++i) {
+          float f[2];
+          Words<T>::unpack(b[t][j][i], f);
+          f[0] *= factor, f[1] *= factor;
+          b[t][j][i] = Words<__half>::pack(f);
         }
-        xsum[t][q][0] = c[0];
-        xsum[t][q][1] = c[1];
-      }
+      undo[t][0] = __shfl_sync(0xffffffffu, inverse, t4 * 8);
+      undo[t][1] = __shfl_sync(0xffffffffu, inverse, t4 * 8 + 4);
+    }
   }
 
   // ---- scales and zero points of a tile's rows g, g + 8, .., asked for a tile ahead where registers allow: two scales and
   // four zero points a register, brought in one load a row where they lie for that
   constexpr int kScW = kGroups / 2, kZpW = (kGroups + 3) / 4;
   constexpr bool kAhead = FL < 4;  // groups of 32 have too many
-  uint32_t scw[2 * RT][kScW], zpw[2 * RT][kZpW], sc_ahead[2 * RT][kScW], zp_ahead[2 * RT][kZpW];
+  uint32_t scw[2 * kHalves][kScW], zpw[2 * kHalves][kZpW], sc_ahead[2 * kHalves][kScW], zp_ahead[2 * kHalves][kZpW];
   auto& scn = kAhead ? sc_ahead : scw;
   auto& zpn = kAhead ? zp_ahead : zpw;
   const auto scale_at = [&](int h, int q) {
@@ -241,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
     const uint8_t* zbase = ZP ? a.z + (int64_t)t * kRows * a.groups : nullptr;
     const int last = a.N - 1 - t * kRows;  // rows past it repeat it, and are not stored
 #pragma unroll
-    for (int h = 0; h < 2 * RT; ++h) {
+    for (int h = 0; h < 2 * kHalves; ++h) {
       const uint32_t row = min(h * 8 + g, last) * a.groups;
       if (a.vec) {
         const T* sp = sbase + (row + goff[0]);
@@ -299,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
   };
   const auto finish = [&](int tr, int parity) {  // the owned units of the round that starts at tile tr
     for (int i = warp; i < places; i += kWarps) {
-      const int u = i * split + rank, t = tr + u / (RT * NT);
+      const int u = i * split + rank, t = tr + u / (kHalves * NT);
       if (u >= kUnits * kRound || t >= t1) continue;
       const float4* from = recv + ((parity * places + i) * split) * 32 + lane;
       float4 v = from[0];
@@ -307,13 +296,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
         const float4 w = from[r * 32];
         v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
       }
-      store(t, u % (RT * NT), v);
+      store(t, u % (kHalves * NT), v);
     }
   };
 
-  const Unpack<T, ZP> unpack;
-  const uint8_t* wlane = smem + warp * kStages * L::kTile + g * (KB * 16) + t4 * 4;
-  const uint32_t turn = (KB == 8 ? g : (g >> 1) & 3) * 16;  // the copy's swizzle of 16-byte blocks
+  const Unpack<ZP> unpack;
+  const uint8_t* wlane = smem + warp * kStages * kTile + g * (kBlocks * 16) + t4 * 4;
+  const uint32_t turn = g * 16;  // the copy's swizzle of 16-byte blocks
   int st = 0, parity = 0, meeting = 0, turns = 0;  // meeting: of the round
   const int inv_split = 65536 / split + 1;  // u inv_split >> 16 is u / split for the few units of a round
   uint32_t phase = 0;
@@ -323,12 +312,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
 #pragma unroll 1
     for (int i = 0; i < kTiles; ++i) {
       const int t = tb + i;
-      float sum[RT][NT][4] = {};
+      float sum[kHalves][NT][4] = {};
       if (active && t < t1) {
         mbar_wait(bars + 8 * st, phase, BRAIN_ERR_TIMEOUT_FULL, 801, abort_flag);
-        const uint8_t* at = wlane + st * L::kTile;
+        const uint8_t* at = wlane + st * kTile;
 #pragma unroll
-        for (int h = 0; kAhead && h < 2 * RT; ++h) {
+        for (int h = 0; kAhead && h < 2 * kHalves; ++h) {
 #pragma unroll
           for (int i = 0; i < kScW; ++i) scw[h][i] = scn[h][i];
           if (ZP)
@@ -338,35 +327,34 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
         if (kAhead && t + 1 < t1) scales(t + 1);
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-          float acc[RT][NT][4];
+          float acc[kHalves][NT][4];
 #pragma unroll
           for (int j = q * kGroupBlocks; j < (q + 1) * kGroupBlocks; ++j) {
             const uint8_t* aj = at + (turn ^ (j * 16));
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
+            for (int r = 0; r < kHalves; ++r) {
               uint32_t w[2][4];
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                unpack(*reinterpret_cast<const uint32_t*>(aj + (r * 2 + h) * 8 * (KB * 16)), ZP ? zero_at(r * 2 + h, q) : 8, w[h]);
+                unpack(*reinterpret_cast<const uint32_t*>(aj + (r * 2 + h) * 8 * (kBlocks * 16)), ZP ? zero_at(r * 2 + h, q) : 8, w[h]);
               const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma<T>(acc[r][n], a0, b[n][j][0], b[n][j][1], j == q * kGroupBlocks);
-                mma<T>(acc[r][n], a1, b[n][j][2], b[n][j][3], false);
+                mma(acc[r][n], a0, b[n][j][0], b[n][j][1], j == q * kGroupBlocks);
+                mma(acc[r][n], a1, b[n][j][2], b[n][j][3], false);
               }
             }
           }
 #pragma unroll
-          for (int h = 0; h < 2 * RT; ++h) {
+          for (int h = 0; h < 2 * kHalves; ++h) {
             const float s = scale_at(h, q);
-            const float off = ZP ? __int_as_float(0xcb000000u | zero_at(h, q)) + (8388608.f - 128.f) : -136.f;  // -128 - z
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 float& to = sum[h / 2][n][h % 2 * 2 + c];
                 const float v = acc[h / 2][n][h % 2 * 2 + c];
-                to = fmaf(s, kSums ? fmaf(off, xsum[n][q][c], v) : v, to);
+                to = fmaf(s, kScaled ? v * undo[n][c] : v, to);
               }
           }
         }
@@ -377,10 +365,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
         phase ^= st == 0;
       }
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+      for (int r = 0; r < kHalves; ++r)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          part[(((i * RT + r) * NT + n) * kWarps + warp) * 32 + lane] =
+          part[(((i * kHalves + r) * NT + n) * kWarps + warp) * 32 + lane] =
               make_float4(sum[r][n][0], sum[r][n][1], sum[r][n][2], sum[r][n][3]);
     }
     // half of the warps, in turn, add up what all of them left; the others go on
@@ -394,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
     if (adds) {
       asm volatile("bar.sync 2, 256;" ::: "memory");
       for (int u = warp % (kWarps / 2); u < kUnits; u += kWarps / 2) {
-        if (tb + u / (RT * NT) >= t1) continue;
+        if (tb + u / (kHalves * NT) >= t1) continue;
         const float4* from = part + u * kWarps * 32 + lane;
         float4 v = from[0];
 #pragma unroll
@@ -408,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
           asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                        : "memory");
         } else {
-          store(tb + u / (RT * NT), u % (RT * NT), v);
+          store(tb + u / (kHalves * NT), u % (kHalves * NT), v);
         }
       }
       __syncwarp();
@@ -417,9 +405,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
       asm volatile("bar.arrive 2, 256;" ::: "memory");
     }
     if (closes) {
-      if (split > 1) {
-        cluster_arrive();
-      }
+      if (split > 1) cluster_arrive();
       meeting = 0;
       parity ^= 1;
     } else {
@@ -432,17 +418,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (RT == 1 ? 3 : 2) : 1)
   }
 }
 
-template <typename T, int NT, int KB, int RT, int FL, bool ZP>
+template <typename T, int NT, int FL, bool ZP>
 int launch_tile(const Int4Args& a, const uint8_t* w, int64_t ldw, cudaStream_t st) {
-  using L = Layout<NT, KB, RT>;
+  using L = Layout<NT>;
   CUtensorMap wmap;
   const uint64_t wd[2] = {(uint64_t)a.K / 2, (uint64_t)a.N}, ws[1] = {(uint64_t)ldw};
-  const uint32_t wb[2] = {KB * 16, L::kRows};
-  if (!brain_host::encode_tiled(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(w), wd, ws, wb,
-                                KB == 8 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+  const uint32_t wb[2] = {kBlocks * 16, kRows};
+  if (!brain_host::encode_tiled(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(w), wd, ws, wb, CU_TENSOR_MAP_SWIZZLE_128B))
     return (int)cudaErrorInvalidValue;
-  const auto kernel = int4_kernel<T, NT, KB, RT, FL, ZP>;
-  const int per = kWarps * KB * 32, split = (a.K + per - 1) / per, tiles = (a.N + L::kRows - 1) / L::kRows;
+  const auto kernel = int4_kernel<T, NT, FL, ZP>;
+  const int per = kWarps * kBlocks * 32, split = (a.K + per - 1) / per, tiles = (a.N + kRows - 1) / kRows;
   const int ntok = (a.M + 8 * NT - 1) / (8 * NT);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads);
@@ -478,8 +463,8 @@ int launch_tile(const Int4Args& a, const uint8_t* w, int64_t ldw, cudaStream_t s
 
 template <typename T, int FL, bool ZP>
 int launch_tokens(const Int4Args& a, const uint8_t* w, int64_t ldw, cudaStream_t st) {
-  if (a.M <= 8) return launch_tile<T, 1, 8, 2, FL, ZP>(a, w, ldw, st);
-  return launch_tile<T, 2, 8, 2, FL, ZP>(a, w, ldw, st);
+  if (a.M <= 8) return launch_tile<T, 1, FL, ZP>(a, w, ldw, st);
+  return launch_tile<T, 2, FL, ZP>(a, w, ldw, st);
 }
 
 template <typename T, bool ZP>

@@ -80,9 +80,8 @@ def dequantize_int4(packed, scales, zeros=None, group_size: int = 128) -> torch.
 
 def int4_linear(x, packed, scales, zeros=None, bias=None, group_size: int = 128) -> torch.Tensor:
     """y = x @ W^T (+ bias) for x [..., K] bf16 or f16 and a packed 4-bit W (:func:`quantize_int4`); scales and
-    bias are of x's type. Values are exact, products and sums f32, and y is rounded once; a bf16 token with an
-    infinite entry (or one above 2^120) gives NaN. The weight is read once for every 16 tokens (8 of up to 8): for
-    few of them. Its rows have to start on 16 bytes. Inference only."""
+    bias are of x's type. Values are exact, products and sums f32, and y is rounded once. The weight is read once for
+    every 16 tokens (8 of up to 8): for few of them. Its rows have to start on 16 bytes. Inference only."""
     N, K = _check_weight(packed, scales, zeros, group_size)
     if x.dim() == 0 or x.shape[-1] != K:
         raise ValueError(f"int4_linear: x {tuple(x.shape)} for a weight [{N}, {K}]")

@@ -147,6 +147,22 @@ def test_non_finite_tokens_stay_in_their_rows():
 
 
 @gpu
+@pytest.mark.parametrize("zeros", [True, False])
+def test_tokens_of_any_size(zeros):
+    # bf16 covers f32's range: each token for itself, and values far below a token's largest
+    packed, scales, z = weight(70, 544, 64, zeros, torch.bfloat16)
+    x = torch.randn(6, 544, generator=torch.Generator().manual_seed(2))
+    x = (x * torch.tensor([2.0 ** -130, 2.0 ** -60, 1, 2.0 ** 60, 2.0 ** 115, 1])[:, None]).bfloat16()
+    x[5, ::2] *= 2.0 ** -20
+    y = Q.int4_linear(x.cuda(), packed.cuda(), scales.cuda(), None if z is None else z.cuda(), group_size=64).cpu()
+    w = dense(packed, scales, z, 64)
+    want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    # as in check, with the smallest step of bf16's range in place of its fixed term
+    tol = 2.0 ** -8 * want.abs() + (544 / 16 + 16) * 2.0 ** -22 * size + 2.0 ** -133
+    assert torch.isfinite(y).all() and ((y.double() - want).abs() <= tol).all()
+
+
+@gpu
 @pytest.mark.parametrize("symmetric", [True, False])
 def test_module(symmetric):
     lin = torch.nn.Linear(512, 96).cuda().bfloat16()
