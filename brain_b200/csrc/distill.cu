@@ -13,11 +13,12 @@
 //
 // Bound by memory: the logits once for the loss; once in and once out for the gradient. A CTA takes a row and, for
 // the gradient, reads it again right after the first pass, out of L2 (or its own ring); the backward pass of autograd
-// has the log-sum-exp and streams pieces of rows. Measured on bf16 rows of 128256: loss of 2048 90 us (5.8 TB/s),
-// gradient alone 165 us (6.4), loss and gradient of 4096 466 us (4.5). Exponentials are not what bounds the last: it
-// took 243 us in place of 254 (for 2048, before the ring) without them. Holding a row on chip for both passes, with a
-// cluster of CTAs, was slower: 560 us with CTAs that load, exchange their sums and store in turn, and 1300 us as a
-// persistent pipeline, whose exchange and entries cost each row several microseconds in a row.
+// has the log-sum-exp and streams pieces of rows. Measured on bf16 rows of 128256: loss of 2048 89 us (5.9 TB/s),
+// gradient alone 165 us (6.4), loss and gradient of 4096 454 us (4.6). Of the last, the second reading costs 58 us and
+// the writing 80; the two exponentials of a value keep their unit 54 % busy, and a CTA's two passes overlap only with
+// the SM's other CTA's. Holding a row on chip for both passes was slower: 586 us with one CTA of 1024 threads an SM, whose
+// ring keeps three quarters of a row, 560 us with clusters of CTAs that load, exchange their sums and store in turn, and
+// 1300 us as a persistent pipeline of those.
 #include <algorithm>
 #include <type_traits>
 
@@ -53,6 +54,24 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two f32 in one operation each.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void one_each(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
 }
 
 // (m, s) += (m2, s2), both log2-domain maxima with sums relative to them
@@ -279,58 +298,12 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
     p[i] = on ? t : -INFINITY;
     zk[i] = on ? to_f32(z[j]) : 0.f;
   }
-  int end = -1;
-  if (tid < sl.head) end = tid;
-  if (tid >= 32 && tid - 32 < a.V - tail) end = tail + tid - 32;
-  float zend = 0.f;
-  if (end >= 0) {
-    zend = to_f32(z[end]);
-    const float f = zend * factor;
-    merge(m, s, f, f == -INFINITY ? 0.f : ex2(f - f));
-  }
-  int slot = 0;
-  for (int block = 0; block < blocks; ++block) {
-    copy_wait<S - 1>();
-    uint32_t w[U * 4];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      uint4 v = ring[(slot * U + u) * kRow];
-      if ((block * U + u) * kRow + tid >= sl.nv) v = make_uint4(kNone, kNone, kNone, kNone);
-      w[u * 4] = v.x, w[u * 4 + 1] = v.y, w[u * 4 + 2] = v.z, w[u * 4 + 3] = v.w;
-    }
-    uint32_t lw = w[0];
-#pragma unroll
-    for (int i = 1; i < U * 4; ++i) lw = max_words<T>(lw, w[i]);
-    float lm[2];
-    W::unpack(lw, lm);
-    if (W::PER == 2) lm[0] = fmaxf(lm[0], lm[1]);
-    const float top2 = fmaxf(m, lm[0] * factor), base = top2 == -INFINITY ? 0.f : top2;
-    s *= m == -INFINITY ? 1.f : ex2(m - base);
-    m = top2;
-    float ls[2] = {};
-#pragma unroll
-    for (int i = 0; i < U * 4; ++i) {
-      float f[2];
-      W::unpack(w[i], f);
-#pragma unroll
-      for (int e = 0; e < W::PER; ++e) ls[e] += ex2(fmaf(f[e], factor, -base));
-    }
-    s += ls[0] + ls[1];
-    if (block + S < blocks) load(block + S, slot);
-    copy_commit();
-    slot = slot == S - 1 ? 0 : slot + 1;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    merge(m, s, m2, s2);
-  }
-  if (lane == 0) {
-    wm[tid / 32] = m;
-    ws[tid / 32] = s;
-  }
-  __syncthreads();
-  if (tid < 32) {  // the teacher's softmax and the loss's own terms
+  // the first warp waits for all entries and makes the teacher's softmax and the loss's own terms, while the others' (and
+  // its own) first blocks are on their way
+  if (tid >= 32) {
+    asm volatile("bar.arrive 1, %0;" ::"n"(kRow) : "memory");
+  } else {
+    asm volatile("bar.sync 1, %0;" ::"n"(kRow) : "memory");
     float top = -INFINITY, sum = 0.f, kl = 0.f;
     bool nan = false;
     for (int i = lane; i < a.k; i += 32) {
@@ -354,6 +327,67 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
       s_kl = kl;
     }
   }
+  int end = -1;
+  if (tid < sl.head) end = tid;
+  if (tid >= 32 && tid - 32 < a.V - tail) end = tail + tid - 32;
+  float zend = 0.f;
+  if (end >= 0) {
+    zend = to_f32(z[end]);
+    const float f = zend * factor;
+    merge(m, s, f, f == -INFINITY ? 0.f : ex2(f - f));
+  }
+  int slot = 0;
+  const uint64_t factor2 = two(factor, factor);
+  const auto take = [&](int block, auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;
+    copy_wait<S - 1>();
+    uint32_t w[U * 4];
+    const uint4* from = ring + slot * U * kRow;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint4 v = from[u * kRow];
+      if (!kWhole && (block * U + u) * kRow + tid >= sl.nv) v = make_uint4(kNone, kNone, kNone, kNone);
+      w[u * 4] = v.x, w[u * 4 + 1] = v.y, w[u * 4 + 2] = v.z, w[u * 4 + 3] = v.w;
+    }
+    uint32_t lw = w[0];
+#pragma unroll
+    for (int i = 1; i < U * 4; ++i) lw = max_words<T>(lw, w[i]);
+    float lm[2];
+    W::unpack(lw, lm);
+    if (W::PER == 2) lm[0] = fmaxf(lm[0], lm[1]);
+    const float top2 = fmaxf(m, lm[0] * factor), base = top2 == -INFINITY ? 0.f : top2;
+    s *= m == -INFINITY ? 1.f : ex2(m - base);
+    m = top2;
+    const uint64_t less = two(-base, -base);
+    uint64_t ls = 0;
+#pragma unroll
+    for (int i = 0; i < U * 4; i += 2 / W::PER) {
+      float f[2];
+      W::unpack(w[i], f);
+      if (W::PER == 1) f[1] = __uint_as_float(w[i + (W::PER == 1)]);
+      one_each(fma2(two(f[0], f[1]), factor2, less), f[0], f[1]);
+      ls = add2(ls, two(ex2(f[0]), ex2(f[1])));
+    }
+    float l0, l1;
+    one_each(ls, l0, l1);
+    s += l0 + l1;
+    if (block + S < blocks) load(block + S, slot);
+    copy_commit();
+    slot = slot == S - 1 ? 0 : slot + 1;
+  };
+  const int full = sl.nv / (U * kRow);
+  for (int block = 0; block < full; ++block) take(block, std::true_type());
+  if (full < blocks) take(full, std::false_type());
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    merge(m, s, m2, s2);
+  }
+  if (lane == 0) {
+    wm[tid / 32] = m;
+    ws[tid / 32] = s;
+  }
+  __syncthreads();
   m = lane < kRow / 32 ? wm[lane] : -INFINITY;
   s = lane < kRow / 32 ? ws[lane] : 0.f;
 #pragma unroll
@@ -362,7 +396,6 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
     merge(m, s, m2, s2);
   }
   const float lse = (m + log2f(s)) * kLn2;
-  __syncthreads();
   const bool any = s_any;
   if (tid == 0) {
     a.loss[row] = any ? a.temp * a.temp * (s_kl + lse) : 0.f;
@@ -375,7 +408,13 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
   T* dz = (T*)a.dz + row * a.lddz;
   const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
   const float g = (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * by * a.temp;
+  if (!any) {  // zeros, also where logits are infinite or NaN
+    for (int i = tid; i < sl.nv; i += kRow) put(dz, sl.head + i * W::N, make_uint4(0, 0, 0, 0), alike);
+    if (end >= 0) dz[end] = from_f32<T>(0.f);
+    return;
+  }
   const float lse2 = lse * kLog2e, shift = log2f(fabsf(g)) - lse2;
+  const uint64_t shift2 = two(shift, shift);
   const uint32_t sign = g < 0.f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
   // what the ring holds first (its oldest block is in `slot`), then the others from the row's start
   const int kept = min(S, blocks);
@@ -390,12 +429,14 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
       const uint4 v = ring[(slot * U + u) * kRow];
       uint4 o;
 #pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
+      for (int e4 = 0; e4 < 4; e4 += 2 / W::PER) {
         float f[2];
         W::unpack(word(v, e4), f);
-#pragma unroll
-        for (int e = 0; e < W::PER; ++e) f[e] = ex2(fmaf(f[e], factor, shift));
-        set_word(o, e4, any ? W::pack(f) ^ sign : 0u);
+        if (W::PER == 1) f[1] = __uint_as_float(word(v, e4 + (W::PER == 1)));
+        one_each(fma2(two(f[0], f[1]), factor2, shift2), f[0], f[1]);
+        f[0] = ex2(f[0]), f[1] = ex2(f[1]);
+        set_word(o, e4, W::pack(f) ^ sign);
+        if (W::PER == 1) set_word(o, e4 + (W::PER == 1), W::pack(f + 1) ^ sign);
       }
       put(dz, sl.head + i * W::N, o, alike);
     }
@@ -403,15 +444,14 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
     copy_commit();
     slot = slot == S - 1 ? 0 : slot + 1;
   }
-  if (end >= 0) dz[end] = from_f32<T>(any ? g * ex2(fmaf(zend, factor, -lse2)) : 0.f);
+  if (end >= 0) dz[end] = from_f32<T>(g * ex2(fmaf(zend, factor, -lse2)));
   __syncthreads();
-  if (any)
-    for (int i = tid; i < a.k; i += kRow) {
-      const int j = id[i];
-      if (j < 0) continue;
-      const float total = first_total(id, p, a.k, i);
-      if (!(total < 0.f)) dz[j] = from_f32<T>(g * (ex2(fmaf(zk[i], factor, -lse2)) - total));
-    }
+  for (int i = tid; i < a.k; i += kRow) {
+    const int j = id[i];
+    if (j < 0) continue;
+    const float total = first_total(id, p, a.k, i);
+    if (!(total < 0.f)) dz[j] = from_f32<T>(g * (ex2(fmaf(zk[i], factor, -lse2)) - total));
+  }
 }
 
 // n[block] = rows of the block's share that have an entry, before the gradient of a mean is written. Most rows have
