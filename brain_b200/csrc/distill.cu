@@ -20,6 +20,7 @@
 // ring keeps three quarters of a row, 560 us with clusters of CTAs that load, exchange their sums and store in turn, and
 // 1300 us as a persistent pipeline of those.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "elem.cuh"
@@ -141,6 +142,12 @@ __device__ __forceinline__ float first_total(const int* ids, const float* p, int
   return total;
 }
 
+// A kept logit over the temperature, at least the lowest finite value: one that overflows is still an entry.
+__device__ __forceinline__ float over_temp(float t, float inv_t) {
+  const float v = t * inv_t;
+  return v == -INFINITY ? -FLT_MAX : v;
+}
+
 // Vector `v` to dz + j: in one store where dz lies on 16 bytes as z does.
 template <typename T>
 __device__ __forceinline__ void put(T* dz, int j, const uint4& v, bool alike) {
@@ -183,8 +190,8 @@ __global__ void __launch_bounds__(kStream) distill_grad_kernel(DistillArgs a, in
     id[i] = -1;
     if (i >= a.k) continue;
     const int64_t j = a.id[row * a.k + i];
-    const float t = a.t[row * a.k + i] * a.inv_t;
-    const bool on = j >= 0 && j < a.V && t != -INFINITY;
+    const float raw = a.t[row * a.k + i], t = over_temp(raw, a.inv_t);
+    const bool on = j >= 0 && j < a.V && raw != -INFINITY;
     const int at = (int)(on ? j : 0), w = (at - sl.head) / W::N;
     const bool mine = on && (at < sl.head ? rank == 0 : at >= tail ? rank == ranks - 1 : w >= sl.v0 && w < sl.v1);
     if (mine) id[i] = at;
@@ -291,9 +298,9 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
     id[i] = -1;
     if (i >= a.k) continue;
     const int64_t j = a.id[row * a.k + i];
-    const float t = a.t[row * a.k + i] * a.inv_t;
+    const float raw = a.t[row * a.k + i], t = over_temp(raw, a.inv_t);
     if (j >= a.V) set_status(BRAIN_ERR_BOUNDS, 711);
-    const bool on = j >= 0 && j < a.V && t != -INFINITY;
+    const bool on = j >= 0 && j < a.V && raw != -INFINITY;
     if (on) id[i] = (int)j;
     p[i] = on ? t : -INFINITY;
     zk[i] = on ? to_f32(z[j]) : 0.f;
@@ -537,7 +544,7 @@ BRAIN_API int brain_distill_rows(int dtype, const void* z, int64_t ldz, const fl
                                  float* lse, float* counts, void* dz, int64_t lddz, const float* grad, const int* n,
                                  int parts, int grad_rows, int64_t M, int k, int V, float temp, cudaStream_t st) {
   if (M <= 0) return 0;
-  if (V <= 0 || k <= 0 || k > kMaxTop || M > INT32_MAX || !(temp > 0.f) || (!loss && (!dz || !lse)))
+  if (V <= 0 || V > (1 << 30) || k <= 0 || k > kMaxTop || M > INT32_MAX || !(temp > 0.f) || (!loss && (!dz || !lse)))
     return (int)cudaErrorInvalidValue;
   const DistillArgs a{z, ldz, t, id, loss, lse, counts, dz, lddz, grad, n, parts, grad_rows, k, V, 1.f / temp, temp};
   switch (dtype) {

@@ -507,7 +507,7 @@ BRAIN_API int brain_int4_linear(int dtype, const void* x, int64_t ldx, const voi
                                 const void* z, const void* bias, void* y, float* sums, int M, int N, int K, int G,
                                 cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || K % 32 || G <= 0 || G % 32 || ldw % 16 || ((uintptr_t)w & 15) || ldx % 8 || ((uintptr_t)x & 15) ||
+  if (N > (1 << 30) || K <= 0 || K % 32 || G <= 0 || G % 32 || ldw % 16 || ((uintptr_t)w & 15) || ldx % 8 || ((uintptr_t)x & 15) ||
       M > 8 * 65535 || K > (1 << 20))
     return (int)cudaErrorInvalidValue;
   const int groups = (K + G - 1) / G;

@@ -226,7 +226,7 @@ BRAIN_API int brain_norm_fp8(int dtype, const void* x, int64_t ldx, const void* 
                              void* sum, void* q, float* scales, int64_t M, int D, int block, float eps,
                              cudaStream_t st) {
   if (M <= 0) return 0;
-  if (D <= 0 || M > INT32_MAX || (block && D % 128)) return (int)cudaErrorInvalidValue;
+  if (D <= 0 || D > (1 << 30) || M > INT32_MAX || (block && D % 128)) return (int)cudaErrorInvalidValue;
   switch (dtype) {
     case BRAIN_BF16: return launch<__nv_bfloat16>(x, ldx, res, ldres, w, sum, q, scales, M, D, block, eps, st);
     case BRAIN_F16: return launch<__half>(x, ldx, res, ldres, w, sum, q, scales, M, D, block, eps, st);

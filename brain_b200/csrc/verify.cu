@@ -295,7 +295,7 @@ BRAIN_API int brain_verify_draft(int dtype, const void* p, int64_t p_seq, int64_
                                  int64_t q_pos, const int64_t* drafted, const int* lens, const float* u, int64_t* out,
                                  int64_t* count, int64_t B, int K, int V, cudaStream_t st) {
   if (B <= 0) return 0;
-  if (V <= 0 || K < 0 || B > 65535) return (int)cudaErrorInvalidValue;
+  if (V <= 0 || V > (1 << 30) || K < 0 || B > 65535) return (int)cudaErrorInvalidValue;
   const VerifyArgs a{p, q, p_seq, p_pos, q_seq, q_pos, drafted, lens, u, out, count, K, V};
   switch (dtype) {
     case BRAIN_BF16: return launch<__nv_bfloat16>(a, B, st);

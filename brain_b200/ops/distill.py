@@ -28,10 +28,10 @@ MAX_TOP = 1024
 def _check(name, logits, teacher_logits, teacher_ids, temperature, reduction):
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"unknown reduction {reduction!r}")
-    if not temperature > 0 or temperature == float("inf"):
-        raise ValueError(f"{name}: temperature {temperature} is not above zero and finite")
-    if logits.dim() == 0 or logits.shape[-1] == 0:
-        raise ValueError(f"{name}: logits {tuple(logits.shape)} have no vocabulary dimension")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"{name}: temperature {temperature} is not in [1e-6, 1e6]")
+    if logits.dim() == 0 or not 0 < logits.shape[-1] <= 2 ** 30:
+        raise ValueError(f"{name}: logits {tuple(logits.shape)} have no vocabulary dimension of 1 to 2^30 ids")
     if teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != logits.shape[:-1] \
             or teacher_ids.dim() != logits.dim():
         raise ValueError(f"{name}: logits {tuple(logits.shape)}, teacher_logits {tuple(teacher_logits.shape)}, "
@@ -119,8 +119,9 @@ def topk_distillation_ref(logits, teacher_logits, teacher_ids, temperature=1.0, 
     V = logits.shape[-1]
     if teacher_ids.numel() and int(teacher_ids.max()) >= V:
         raise ValueError(f"teacher id {int(teacher_ids.max())} outside the vocabulary of {V}")
-    t = teacher_logits.detach().to(ct) / temperature
+    t = teacher_logits.detach().to(ct)
     on = (teacher_ids >= 0) & (t != float("-inf"))
+    t = (t / temperature).clamp_min(torch.finfo(ct).min)  # one that overflows is still an entry
     some = on.any(-1)
     t = torch.where(on, t, torch.full_like(t, float("-inf")))
     t = torch.where(some[..., None], t, torch.zeros_like(t))

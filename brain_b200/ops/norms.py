@@ -175,8 +175,9 @@ def _norm_fp8(name, x, r, w, eps, scaling):
     if scaling not in ("rowwise", "block"):
         raise ValueError(f"unknown fp8 scaling {scaling!r}")
     D = x.shape[-1] if x.dim() else 0
-    if D == 0 or (scaling == "block" and D % 128):
-        raise ValueError(f"{name}: last dimension {D}" + (" is not a multiple of 128" if D else ""))
+    if not 0 < D <= 2 ** 30 or (scaling == "block" and D % 128):
+        raise ValueError(f"{name}: last dimension {D} is not " +
+                         ("a multiple of 128" if 0 < D <= 2 ** 30 else "one of 1 to 2^30"))
     if w.shape != (D,) or (r is not None and r.shape != x.shape):
         raise ValueError(f"{name}: x {tuple(x.shape)}, residual {None if r is None else tuple(r.shape)}, "
                          f"weight {tuple(w.shape)}")

@@ -11,8 +11,8 @@ from ._common import dtype_code, launch, ptr, same_device
 def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_lens=None):
     """Which drafted tokens the target's probabilities accept -> (tokens [B, K + 1], accepted [B]), int64.
 
-    ``target_probs`` [B, K + 1, V] (up to 65535 sequences): the target's probabilities after the context and each drafted token;
-    ``draft_tokens`` [B, K]; ``draft_probs`` [B, K, V]: what each token was drawn from (None: the draft was
+    ``target_probs`` [B, K + 1, V] (up to 65535 sequences and 2^30 ids): the target's probabilities after the
+    context and each drafted token; ``draft_tokens`` [B, K]; ``draft_probs`` [B, K, V]: what each token was drawn from (None: the draft was
     certain of its tokens); ``draft_lens`` [B]: how many of the K were drafted (None: all); ``uniforms``
     [B, K + 1] in [0, 1): one number a drafted token, the last for the token that follows.
 
@@ -25,7 +25,7 @@ def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_l
         raise ValueError("verify_draft takes target_probs [B, K + 1, V] and draft_tokens [B, K]")
     B, K1, V = target_probs.shape
     K = K1 - 1
-    if V == 0 or K < 0 or B > 65535 or draft_tokens.shape != (B, K) or uniforms.shape != (B, K1):
+    if not 0 < V <= 2 ** 30 or K < 0 or B > 65535 or draft_tokens.shape != (B, K) or uniforms.shape != (B, K1):
         raise ValueError(f"verify_draft: target_probs {tuple(target_probs.shape)}, draft_tokens "
                          f"{tuple(draft_tokens.shape)}, uniforms {tuple(uniforms.shape)}")
     if draft_probs is not None and draft_probs.shape != (B, K, V):
@@ -56,8 +56,8 @@ def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_l
     tokens = drafted.new_empty((B, K1))
     count = drafted.new_empty(B)
     ps, qs = p.stride(), (0, 0) if q is None else q.stride()
-    launch(p, "brain_verify_draft", code, p.data_ptr(), ps[0], ps[1], ptr(q), qs[0], qs[1], drafted.data_ptr(), ptr(lens),
-           u.data_ptr(), tokens.data_ptr(), count.data_ptr(), B, K, V)
+    launch(p, "brain_verify_draft", code, p.data_ptr(), ps[0], ps[1], ptr(q), qs[0], qs[1], drafted.data_ptr(),
+           ptr(lens), u.data_ptr(), tokens.data_ptr(), count.data_ptr(), B, K, V)
     return tokens, count
 
 

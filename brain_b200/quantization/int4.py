@@ -59,6 +59,8 @@ def _check_weight(packed, scales, zeros, group_size):
     if packed.dim() != 2 or packed.dtype != torch.uint8:
         raise ValueError(f"packed int4 weight: [N, K / 2] uint8 is needed, not {tuple(packed.shape)} {packed.dtype}")
     N, K = packed.shape[0], packed.shape[1] * 2
+    if N > 2 ** 30:
+        raise ValueError(f"packed int4 weight: {N} output features, 2^30 are taken")
     _check_group(K, group_size)
     groups = -(-K // group_size)
     if scales.shape != (N, groups) or (zeros is not None and zeros.shape != (N, groups)):

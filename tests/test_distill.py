@@ -100,6 +100,22 @@ def test_gradient_against_differences():
     assert torch.autograd.gradcheck(lambda v: ops.topk_distillation(v, t, ids, 1.7), (z,))
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_teacher_masked_with_the_lowest_value(device, reduction):
+    # below one, the temperature takes it out of f32's range: an entry all the same, where it is the only one
+    z, t, ids = data(4, 40, 5, torch.float32)
+    t[0, 1:] = t[1] = torch.finfo(torch.float32).min
+    ids[1, 1:] = -1
+    ids[2] = -1
+    loss, grad = ops.topk_distillation_grad(z.to(device), t.to(device), ids.to(device), 0.5, reduction)
+    check(loss, grad, z, t, ids, 0.5, reduction, torch.float32)
+    v = z.to(device).requires_grad_()
+    loss = ops.topk_distillation(v, t.to(device), ids.to(device), 0.5, reduction)
+    (grad,) = torch.autograd.grad(loss.sum(), v)
+    check(loss, grad, z, t, ids, 0.5, reduction, torch.float32)
+
+
 def test_is_distillation_loss_when_everything_is_kept():
     z, teacher = torch.randn(5, 16), torch.randn(5, 16)
     ids = torch.arange(16).expand(5, 16)
@@ -117,6 +133,11 @@ def test_refusals():
                 dict(reduction="batchmean")):
         with pytest.raises(ValueError):
             ops.topk_distillation(z, t, ids, **bad)
+    for temperature in (1e-7, 1e-50, 1e7):
+        with pytest.raises(ValueError):
+            ops.topk_distillation(z, t, ids, temperature)
+    with pytest.raises(ValueError):
+        ops.topk_distillation(z[:1, :1].expand(1, 2 ** 30 + 1), t[:1], ids[:1])
     for a in ((z, t[:, :3], ids), (z[:2], t, ids), (z, t[:, :0], ids[:, :0]), (z[:, :0], t, ids), (z[None], t, ids),
               (z, t.repeat(1, 300), ids.repeat(1, 300))):
         with pytest.raises(ValueError):

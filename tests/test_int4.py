@@ -75,6 +75,8 @@ def test_refusals():
                 lambda: Q.int4_linear(x, packed, scales, z, group_size=48),
                 lambda: Q.int4_linear(x, packed, scales, z, torch.zeros(7).bfloat16(), 64),
                 lambda: Q.int4_linear(x, packed.int(), scales, z, group_size=64),
+                lambda: Q.int4_linear(x, packed[:1, :1].expand(2 ** 30 + 1, 64), scales[:1, :1].expand(2 ** 30 + 1, 2),
+                                      group_size=64),
                 lambda: Q.quantize_int4(torch.zeros(4, 48), 32),
                 lambda: Q.quantize_int4(torch.zeros(1, 96 * 384), 96),
                 lambda: Q.quantize_int4(torch.zeros(64), 32)):

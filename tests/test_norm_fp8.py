@@ -58,6 +58,8 @@ def test_refusals():
         ops.rms_norm_fp8(x, w[:95])
     with pytest.raises(ValueError):
         ops.rms_norm_fp8(x[:, :0], w[:0])
+    with pytest.raises(ValueError):
+        ops.rms_norm_fp8(x[:1, :1].expand(1, 2 ** 30 + 128), w[:1].expand(2 ** 30 + 128))
     with pytest.raises(TypeError):
         ops.rms_norm_fp8(x, w.float())
     with pytest.raises(TypeError):

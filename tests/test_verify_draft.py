@@ -54,7 +54,8 @@ def test_samples_are_the_targets():
 def test_refusals():
     p, x, u, q = data(2, 3, 10)
     for bad in ((p[0], x, u, q), (p, x[:, :2], u, q), (p, x, u[:, :3], q), (p, x, u, q[..., :9]),
-                (p, x, u, q, torch.zeros(3, dtype=torch.int32)), (p[..., :0], x, u, q[..., :0]), (p[:, :0], x, u)):
+                (p, x, u, q, torch.zeros(3, dtype=torch.int32)), (p[..., :0], x, u, q[..., :0]), (p[:, :0], x, u),
+                (p[:1, :1, :1].expand(1, 1, 2 ** 30 + 1), x[:1, :0], u[:1, :1])):
         with pytest.raises(ValueError):
             ops.verify_draft(*bad)
     for bad in ((p.double(), x, u, q.double()), (p, x.float(), u, q), (p, x, u.double(), q), (p, x, u, q.half()),
