@@ -537,24 +537,6 @@ int launch(const DistillArgs& a, int64_t M, cudaStream_t st) {
 
 BRAIN_STATUS_READER(distill)
 
-// Rows: loss [M] (null: take lse), lse [M] (may be null with loss), counts [M] (may be null), dz (null: none; may
-// be z) with its row stride. The gradient is scaled by grad (null: 1; one a row with
-// grad_rows) and divided by the sum of n's parts (null: no division).
-BRAIN_API int brain_distill_rows(int dtype, const void* z, int64_t ldz, const float* t, const int64_t* id, float* loss,
-                                 float* lse, float* counts, void* dz, int64_t lddz, const float* grad, const int* n,
-                                 int parts, int grad_rows, int64_t M, int k, int V, float temp, cudaStream_t st) {
-  if (M <= 0) return 0;
-  if (V <= 0 || V > (1 << 30) || k <= 0 || k > kMaxTop || M > INT32_MAX || !(temp > 0.f) || (!loss && (!dz || !lse)))
-    return (int)cudaErrorInvalidValue;
-  const DistillArgs a{z, ldz, t, id, loss, lse, counts, dz, lddz, grad, n, parts, grad_rows, k, V, 1.f / temp, temp};
-  switch (dtype) {
-    case BRAIN_BF16: return launch<__nv_bfloat16>(a, M, st);
-    case BRAIN_F16: return launch<__half>(a, M, st);
-    case BRAIN_F32: return launch<float>(a, M, st);
-  }
-  return (int)cudaErrorInvalidValue;
-}
-
 // n [parts]: the rows with an entry, share by share.
 BRAIN_API int brain_distill_count(const float* t, const int64_t* id, int64_t M, int k, int V, int* n, int parts,
                                   cudaStream_t st) {
@@ -567,4 +549,33 @@ BRAIN_API int brain_distill_reduce(const float* loss, const float* counts, int64
                                    cudaStream_t st) {
   distill_reduce_kernel<<<1, 1024, 0, st>>>(loss, counts, M, n, parts, total);
   return (int)cudaGetLastError();
+}
+
+// Rows: loss [M] (null: take lse), lse [M] (may be null with loss), counts [M] (may be null), dz (null: none; may
+// be z) with its row stride. The gradient is scaled by grad (null: 1; one a row with
+// grad_rows) and divided by the sum of n's parts (null: no division), which are counted first with `count`. Where total
+// is given, brain_distill_reduce follows (all in one call, as a call from Python costs as much as a small kernel).
+BRAIN_API int brain_distill_rows(int dtype, const void* z, int64_t ldz, const float* t, const int64_t* id, float* loss,
+                                 float* lse, float* counts, void* dz, int64_t lddz, const float* grad, int* n,
+                                 int parts, int count, int grad_rows, int64_t M, int k, int V, float temp, float* total,
+                                 cudaStream_t st) {
+  if (M < 0 || V <= 0 || V > (1 << 30) || k <= 0 || k > kMaxTop || M > INT32_MAX || !(temp > 0.f) ||
+      (M > 0 && !loss && (!dz || !lse || total)))
+    return (int)cudaErrorInvalidValue;
+  if (count) {
+    const int e = brain_distill_count(t, id, M, k, V, n, parts, st);
+    if (e) return e;
+  }
+  const DistillArgs a{z, ldz, t, id, loss, lse, counts, dz, lddz, grad, dz ? n : nullptr, parts, grad_rows, k, V,
+                      1.f / temp, temp};
+  if (M > 0) {
+    int e = (int)cudaErrorInvalidValue;
+    switch (dtype) {
+      case BRAIN_BF16: e = launch<__nv_bfloat16>(a, M, st); break;
+      case BRAIN_F16: e = launch<__half>(a, M, st); break;
+      case BRAIN_F32: e = launch<float>(a, M, st); break;
+    }
+    if (e) return e;
+  }
+  return total ? brain_distill_reduce(loss, counts, M, n, parts, total, st) : 0;
 }

@@ -49,7 +49,7 @@ _native.register({
     "brain_status_optim": ("brain_kernels", "pi"),
     "brain_status_attention": ("brain_kernels", "pi"),
     "brain_norm_fp8": ("brain_kernels", "iplplppppliifs"),
-    "brain_distill_rows": ("brain_kernels", "iplpppppplppiiliifs"),
+    "brain_distill_rows": ("brain_kernels", "iplpppppplppiiiliifps"),
     "brain_distill_count": ("brain_kernels", "ppliipis"),
     "brain_distill_reduce": ("brain_kernels", "pplpips"),
     "brain_status_distill": ("brain_kernels", "pi"),

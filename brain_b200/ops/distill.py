@@ -57,24 +57,23 @@ def _teacher(teacher_logits, teacher_ids):
     return t, ids
 
 
-def _rows(l2, t, ids, temperature, loss, lse, counts, dz, grad=None, n=None, grad_rows=False):
+def _rows(l2, t, ids, temperature, loss, lse, counts, dz, grad=None, n=None, grad_rows=False, count=False, total=None):
     launch(l2, "brain_distill_rows", DTYPE_CODES[l2.dtype], l2.data_ptr(), l2.stride(0), t.data_ptr(), ids.data_ptr(),
            ptr(loss), ptr(lse), ptr(counts), ptr(dz), 0 if dz is None else dz.stride(0), ptr(grad), ptr(n),
-           0 if n is None else n.numel(), int(grad_rows), l2.shape[0], t.shape[-1], l2.shape[1], temperature)
+           0 if n is None else n.numel(), int(count), int(grad_rows), l2.shape[0], t.shape[-1], l2.shape[1], temperature,
+           ptr(total))
+
+
+def _parts(t, M):
+    """Room for the numbers of the tokens that have an entry."""
+    return t.new_empty(min(max(-(-M // 256), 1), 128), dtype=torch.int32)
 
 
 def _count(t, ids, M, V):
     """Numbers of the tokens that have an entry, in parts."""
-    n = t.new_empty(min(max(-(-M // 256), 1), 128), dtype=torch.int32)
+    n = _parts(t, M)
     launch(t, "brain_distill_count", t.data_ptr(), ids.data_ptr(), M, t.shape[-1], V, n.data_ptr(), n.numel())
     return n
-
-
-def _total(loss, counts, n):
-    total = loss.new_empty(())
-    launch(loss, "brain_distill_reduce", loss.data_ptr(), ptr(counts), loss.shape[-1], ptr(n),
-           0 if n is None else n.numel(), total.data_ptr())
-    return total
 
 
 def _loss(l2, t, ids, temperature, reduction, lse=None, n=None):
@@ -82,11 +81,12 @@ def _loss(l2, t, ids, temperature, reduction, lse=None, n=None):
     M = l2.shape[0]
     if reduction != "mean":
         loss = t.new_empty(M)
-        _rows(l2, t, ids, temperature, loss, lse, None, None)
-        return loss if reduction == "none" else _total(loss, None, None)
-    loss = t.new_empty((2, M))
-    _rows(l2, t, ids, temperature, loss, lse, loss[1], None)
-    return _total(loss, loss[1], n)
+        total = None if reduction == "none" else t.new_empty(())
+        _rows(l2, t, ids, temperature, loss, lse, None, None, total=total)
+        return loss if reduction == "none" else total
+    loss, total = t.new_empty((2, M)), t.new_empty(())
+    _rows(l2, t, ids, temperature, loss, lse, loss[1], None, n=n, total=total)
+    return total
 
 
 class _DistillFn(torch.autograd.Function):
@@ -193,11 +193,12 @@ def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: flo
         if out is None:
             out = torch.empty_like(logits, memory_format=torch.contiguous_format)
         o2 = out if out.dim() == 2 else out.view(-1, out.shape[-1])
-        M, V = l2.shape
-        n = _count(t, ids, M, V) if reduction == "mean" else None
+        M = l2.shape[0]
         loss = t.new_empty(M)
-        _rows(l2, t, ids, float(temperature), loss, None, None, o2, None, n)
-        return (loss.view(logits.shape[:-1]) if reduction == "none" else _total(loss, None, n)), out
+        n = _parts(t, M) if reduction == "mean" else None
+        total = None if reduction == "none" else t.new_empty(())
+        _rows(l2, t, ids, float(temperature), loss, None, None, o2, None, n, count=n is not None, total=total)
+        return (loss.view(logits.shape[:-1]) if reduction == "none" else total), out
 
 
 class _LinearDistillFn(torch.autograd.Function):
@@ -217,7 +218,9 @@ class _LinearDistillFn(torch.autograd.Function):
             _rows(dlogits[rows], t[rows], ids[rows], temperature, loss[rows], None, None, dlogits[rows], None, n)
         ctx.save_for_backward(h2, w, dlogits)
         ctx.hshape = h.shape
-        return _total(loss, None, n)
+        total = loss.new_empty(())
+        launch(loss, "brain_distill_reduce", loss.data_ptr(), None, M, n.data_ptr(), n.numel(), total.data_ptr())
+        return total
 
     @staticmethod
     @once_differentiable
