@@ -521,14 +521,18 @@ int launch(const DistillArgs& a, int64_t M, cudaStream_t st) {
     kernel<<<(unsigned)M, threads, ring + smem, st>>>(a);
     return (int)cudaGetLastError();
   };
-  // Short rows are bound by what a row costs besides its values, so many small CTAs share an SM; long ones, and few
-  // of them, by what one CTA has in flight (8192 x 4000 bf16: 79 us with 128 threads, 128 with 256, 232 with 512;
-  // 2048 x 50257: 115, 109, 134; 4096 x 128256: 575, 535, 466).
+  // Short rows are bound by what a row costs besides its values, so many small CTAs share an SM (64 threads where there are
+  // more rows than CTAs of 128 run at once); long ones, and few of them, by what one CTA has in flight. Loss and gradient,
+  // bf16, with 64, 128, 256 and 512 threads: 8192 x 4000 61, 75, 125, 225 us; 4096 x 16000 73, 80, 97, -; 3000 x 24000 90, 84, 91,
+  // 126; 3000 x 32000 119, 112, 108, 134; 2048 x 50257 -, 115, 104, 127; 4096 x 128256 -, 559, 525, 440; 300 x 4000 12.3, 11.7,
+  // 12.3, 16.1; 30 x 100000 43, 27, 22, 22.
+  const int sms = brain_host::num_sms();
   const auto pick = [&](auto grad) {
     constexpr bool kGrad = decltype(grad)::value;
-    if (bytes > 131072 || M <= brain_host::num_sms()) return run(distill_row_kernel<T, kGrad, 512, 4, 3, 2>, 512, 512 * 4 * 3 * 16);
-    if (bytes > 16384) return run(distill_row_kernel<T, kGrad, 256, 4, 3, 4>, 256, 256 * 4 * 3 * 16);
-    return run(distill_row_kernel<T, kGrad, 128, 4, 3, 8>, 128, 128 * 4 * 3 * 16);
+    if (bytes > 131072 || M <= sms) return run(distill_row_kernel<T, kGrad, 512, 4, 3, 2>, 512, 512 * 4 * 3 * 16);
+    if (bytes > 49152) return run(distill_row_kernel<T, kGrad, 256, 4, 3, 4>, 256, 256 * 4 * 3 * 16);
+    if (bytes > 32768 || M <= 8 * sms) return run(distill_row_kernel<T, kGrad, 128, 4, 2, 8>, 128, 128 * 4 * 2 * 16);
+    return run(distill_row_kernel<T, kGrad, 64, 4, 2, 16>, 64, 64 * 4 * 2 * 16);
   };
   return a.dz ? pick(std::true_type()) : pick(std::false_type());
 }

@@ -170,7 +170,7 @@ def test_refusals():
 @pytest.mark.parametrize("rows,V,k,T", [
     (1, 1, 1, 1.0), (3, 7, 7, 2.0), (2, 33, 1, 0.5), (5, 1000, 20, 1.0), (4, 1003, 64, 4.0), (3, 32000, 128, 1.0),
     (2, 50257, 100, 2.0), (2, 128256, 256, 1.0), (1, 128256, 1024, 1.5), (2, 200003, 5, 1.0), (200, 515, 9, 1.0),
-    (1, 900001, 3, 1.0), (301, 33000, 7, 1.0), (170, 50257, 20, 2.0), (160, 128256, 5, 1.0),
+    (1, 900001, 3, 1.0), (1300, 130, 5, 1.0), (1200, 4003, 2, 1.5), (301, 33000, 7, 1.0), (170, 50257, 20, 2.0), (160, 128256, 5, 1.0),
     (0, 64, 4, 1.0)])
 def test_loss_and_gradients(dtype, rows, V, k, T):
     z, t, ids = data(rows, V, k, dtype, rows + V)
