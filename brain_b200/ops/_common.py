@@ -65,8 +65,9 @@ STATUS_TAGS = ["gemm", "norms", "elementwise", "ce", "optim", "attention", "atte
 def same_device(ref: torch.Tensor, *others) -> None:
     """Raise unless every tensor in ``others`` (None skipped) lives on ``ref``'s device: a kernel given a
     pointer into another device's (or the host's) memory would fault."""
+    device = ref.device
     for t in others:
-        if t is not None and t.device != ref.device:
+        if t is not None and t.device != device:
             raise ValueError(f"tensor on {t.device} passed to a kernel running on {ref.device}")
 
 

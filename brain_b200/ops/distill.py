@@ -30,36 +30,38 @@ def _check(name, logits, teacher_logits, teacher_ids, temperature, reduction):
         raise ValueError(f"unknown reduction {reduction!r}")
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"{name}: temperature {temperature} is not in [1e-6, 1e6]")
-    if logits.dim() == 0 or not 0 < logits.shape[-1] <= 2 ** 30:
-        raise ValueError(f"{name}: logits {tuple(logits.shape)} have no vocabulary dimension of 1 to 2^30 ids")
-    if teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != logits.shape[:-1] \
-            or teacher_ids.dim() != logits.dim():
-        raise ValueError(f"{name}: logits {tuple(logits.shape)}, teacher_logits {tuple(teacher_logits.shape)}, "
-                         f"teacher_ids {tuple(teacher_ids.shape)}")
-    if not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
-        raise ValueError(f"{name}: {teacher_ids.shape[-1]} teacher entries a token, 1 to {MAX_TOP} are taken")
-    if teacher_ids.is_floating_point() or teacher_ids.is_complex() or teacher_ids.dtype == torch.bool:
+    shape, kept = logits.shape, teacher_ids.shape
+    if not shape or not 0 < shape[-1] <= 2 ** 30:
+        raise ValueError(f"{name}: logits {tuple(shape)} have no vocabulary dimension of 1 to 2^30 ids")
+    if teacher_logits.shape != kept or len(kept) != len(shape) or kept[:-1] != shape[:-1]:
+        raise ValueError(f"{name}: logits {tuple(shape)}, teacher_logits {tuple(teacher_logits.shape)}, "
+                         f"teacher_ids {tuple(kept)}")
+    if not 1 <= kept[-1] <= MAX_TOP:
+        raise ValueError(f"{name}: {kept[-1]} teacher entries a token, 1 to {MAX_TOP} are taken")
+    if teacher_ids.dtype is not torch.int64 and (
+            teacher_ids.is_floating_point() or teacher_ids.is_complex() or teacher_ids.dtype is torch.bool):
         raise TypeError(f"{name}: teacher_ids are whole numbers")
-    if not teacher_logits.is_floating_point():
+    if teacher_logits.dtype is not torch.float32 and not teacher_logits.is_floating_point():
         raise TypeError(f"{name}: teacher_logits are floating-point numbers")
-    if torch.is_grad_enabled() and teacher_logits.requires_grad:
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} gives the teacher no gradient: detach teacher_logits")
     same_device(logits, teacher_logits, teacher_ids)
 
 
 def _teacher(teacher_logits, teacher_ids):
     """The entries as contiguous float32 and int64 (their leading dimensions do not matter to the kernels)."""
-    t, ids = teacher_logits.detach(), teacher_ids
-    if t.dtype != torch.float32 or not t.is_contiguous():
+    t, ids = teacher_logits, teacher_ids
+    if t.dtype is not torch.float32 or not t.is_contiguous():
         t = t.float().contiguous()
-    if ids.dtype != torch.int64 or not ids.is_contiguous():
+    if ids.dtype is not torch.int64 or not ids.is_contiguous():
         ids = ids.long().contiguous()
     return t, ids
 
 
 def _rows(l2, t, ids, temperature, loss, lse, counts, dz, grad=None, n=None, grad_rows=False, count=False, total=None):
+    """``counts`` is an address."""
     launch(l2, "brain_distill_rows", DTYPE_CODES[l2.dtype], l2.data_ptr(), l2.stride(0), t.data_ptr(), ids.data_ptr(),
-           ptr(loss), ptr(lse), ptr(counts), ptr(dz), 0 if dz is None else dz.stride(0), ptr(grad), ptr(n),
+           ptr(loss), ptr(lse), counts, ptr(dz), 0 if dz is None else dz.stride(0), ptr(grad), ptr(n),
            0 if n is None else n.numel(), int(count), int(grad_rows), l2.shape[0], t.shape[-1], l2.shape[1], temperature,
            ptr(total))
 
@@ -84,8 +86,8 @@ def _loss(l2, t, ids, temperature, reduction, lse=None, n=None):
         total = None if reduction == "none" else t.new_empty(())
         _rows(l2, t, ids, temperature, loss, lse, None, None, total=total)
         return loss if reduction == "none" else total
-    loss, total = t.new_empty((2, M)), t.new_empty(())
-    _rows(l2, t, ids, temperature, loss, lse, loss[1], None, n=n, total=total)
+    loss, total = t.new_empty(2 * M), t.new_empty(())  # the losses, then which tokens count
+    _rows(l2, t, ids, temperature, loss, lse, loss.data_ptr() + 4 * M if M else None, None, n=n, total=total)
     return total
 
 
@@ -187,18 +189,19 @@ def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: flo
             grad = torch.autograd.grad(loss.sum(), z)[0]
         return loss.detach(), grad if out is None else out.copy_(grad)
     dtype_code(name, logits)
-    with torch.no_grad():
-        t, ids = _teacher(teacher_logits, teacher_ids)
-        l2 = rows2d(logits)
-        if out is None:
-            out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-        o2 = out if out.dim() == 2 else out.view(-1, out.shape[-1])
-        M = l2.shape[0]
-        loss = t.new_empty(M)
-        n = _parts(t, M) if reduction == "mean" else None
-        total = None if reduction == "none" else t.new_empty(())
-        _rows(l2, t, ids, float(temperature), loss, None, None, o2, None, n, count=n is not None, total=total)
-        return (loss.view(logits.shape[:-1]) if reduction == "none" else total), out
+    if logits.requires_grad:
+        logits = logits.detach()
+    t, ids = _teacher(teacher_logits, teacher_ids)
+    l2 = rows2d(logits)
+    if out is None:
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    o2 = out if out.dim() == 2 else out.detach().view(-1, out.shape[-1])
+    M = l2.shape[0]
+    loss = t.new_empty(M)
+    n = _parts(t, M) if reduction == "mean" else None
+    total = None if reduction == "none" else t.new_empty(())
+    _rows(l2, t, ids, float(temperature), loss, None, None, o2, None, n, count=n is not None, total=total)
+    return (loss.view(logits.shape[:-1]) if reduction == "none" else total), out
 
 
 class _LinearDistillFn(torch.autograd.Function):

@@ -174,14 +174,15 @@ def rms_norm_fp8_ref(s, w, eps, scaling):
 def _norm_fp8(name, x, r, w, eps, scaling):
     if scaling not in ("rowwise", "block"):
         raise ValueError(f"unknown fp8 scaling {scaling!r}")
-    D = x.shape[-1] if x.dim() else 0
+    shape = x.shape
+    D = shape[-1] if shape else 0
     if not 0 < D <= 2 ** 30 or (scaling == "block" and D % 128):
         raise ValueError(f"{name}: last dimension {D} is not " +
                          ("a multiple of 128" if 0 < D <= 2 ** 30 else "one of 1 to 2^30"))
-    if w.shape != (D,) or (r is not None and r.shape != x.shape):
+    if w.shape != (D,) or (r is not None and r.shape != shape):
         raise ValueError(f"{name}: x {tuple(x.shape)}, residual {None if r is None else tuple(r.shape)}, "
                          f"weight {tuple(w.shape)}")
-    if w.dtype != x.dtype or (r is not None and r.dtype != x.dtype):
+    if w.dtype is not x.dtype or (r is not None and r.dtype is not x.dtype):
         raise TypeError(f"{name}: x, the residual and the weight are of one type")
     code = dtype_code(name, x)
     no_backward(name, x, r, w)
