@@ -100,8 +100,10 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 def no_backward(name: str, *tensors) -> None:
     """Raise when autograd would record an inference op: its result would carry no gradient, silently."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def stream(t: torch.Tensor) -> int:

@@ -58,61 +58,58 @@ def _teacher(teacher_logits, teacher_ids):
     return t, ids
 
 
-def _rows(l2, t, ids, temperature, loss, lse, counts, dz, grad=None, n=None, grad_rows=False, count=False, total=None):
-    """``counts`` is an address."""
+def _rows(l2, t, ids, temperature, loss, lse, counts, dz, grad=None, n=None, parts=0, grad_rows=0, count=0, total=None):
+    """All but logits, entries and ``dz`` are addresses; those of empty tensors are None or never used."""
     launch(l2, "brain_distill_rows", DTYPE_CODES[l2.dtype], l2.data_ptr(), l2.stride(0), t.data_ptr(), ids.data_ptr(),
-           ptr(loss), ptr(lse), counts, ptr(dz), 0 if dz is None else dz.stride(0), ptr(grad), ptr(n),
-           0 if n is None else n.numel(), int(count), int(grad_rows), l2.shape[0], t.shape[-1], l2.shape[1], temperature,
-           ptr(total))
+           loss, lse, counts, ptr(dz), 0 if dz is None else dz.stride(0), grad, n, parts, count, grad_rows, l2.shape[0],
+           t.shape[-1], l2.shape[1], temperature, total)
 
 
-def _parts(t, M):
-    """Room for the numbers of the tokens that have an entry."""
-    return t.new_empty(min(max(-(-M // 256), 1), 128), dtype=torch.int32)
+def _parts(M):
+    """In how many parts the tokens that have an entry are counted."""
+    return min(max(-(-M // 256), 1), 128)
 
 
-def _count(t, ids, M, V):
-    """Numbers of the tokens that have an entry, in parts."""
-    n = _parts(t, M)
-    launch(t, "brain_distill_count", t.data_ptr(), ids.data_ptr(), M, t.shape[-1], V, n.data_ptr(), n.numel())
-    return n
-
-
-def _loss(l2, t, ids, temperature, reduction, lse=None, n=None):
-    """The loss; where given, ``lse`` [M] and (of a mean) ``n`` [1] are written too."""
+def _loss(l2, t, ids, temperature, reduction):
+    """The loss, and a buffer whose second and last parts the backward pass reads: losses [M], log-sum-exps [M], which
+    tokens count [M], how many do [1] (an int32)."""
     M = l2.shape[0]
-    if reduction != "mean":
+    own = t.new_empty(3 * M + 1)
+    at = own.data_ptr()
+    if reduction == "none":
         loss = t.new_empty(M)
-        total = None if reduction == "none" else t.new_empty(())
-        _rows(l2, t, ids, temperature, loss, lse, None, None, total=total)
-        return loss if reduction == "none" else total
-    loss, total = t.new_empty(2 * M), t.new_empty(())  # the losses, then which tokens count
-    _rows(l2, t, ids, temperature, loss, lse, loss.data_ptr() + 4 * M if M else None, None, n=n, total=total)
-    return total
+        _rows(l2, t, ids, temperature, loss.data_ptr(), at + 4 * M, None, None)
+        return loss, own
+    total = t.new_empty(())
+    mean = reduction == "mean"
+    _rows(l2, t, ids, temperature, at, at + 4 * M, at + 8 * M if mean else None, None, None, at + 12 * M if mean else None,
+          1 if mean else 0, total=total.data_ptr())
+    return total, own
 
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, t, ids, temperature, reduction):
-        l2 = rows2d(logits)
-        lse = t.new_empty(l2.shape[0])
-        n = t.new_empty(1, dtype=torch.int32) if reduction == "mean" else None
-        loss = _loss(l2, t, ids, temperature, reduction, lse, n)
-        ctx.save_for_backward(logits, t, ids, lse, n)
+        loss, own = _loss(rows2d(logits), t, ids, temperature, reduction)
+        ctx.save_for_backward(logits, t, ids, own)
         ctx.meta = temperature, reduction
         return loss.view(logits.shape[:-1]) if reduction == "none" else loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        logits, t, ids, lse, n = ctx.saved_tensors
+        logits, t, ids, own = ctx.saved_tensors
         temperature, reduction = ctx.meta
         l2 = rows2d(logits)
+        M = l2.shape[0]
         out = torch.empty_like(l2, memory_format=torch.contiguous_format)
-        if g.dtype != torch.float32 or not g.is_contiguous():
+        if g.dtype is not torch.float32 or not g.is_contiguous():
             g = g.float().contiguous()
-        _rows(l2, t, ids, temperature, None, lse, None, out, g, n, grad_rows=reduction == "none")
-        return out.view(logits.shape), None, None, None, None
+        at = own.data_ptr()
+        mean = reduction == "mean"
+        _rows(l2, t, ids, temperature, None, at + 4 * M, None, out, g.data_ptr(), at + 12 * M if mean else None,
+              1 if mean else 0, 1 if reduction == "none" else 0)
+        return out if l2 is logits else out.view(logits.shape), None, None, None, None
 
 
 def topk_distillation_ref(logits, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
@@ -150,7 +147,7 @@ def topk_distillation(logits, teacher_logits, teacher_ids, temperature: float = 
     t, ids = _teacher(teacher_logits, teacher_ids)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillFn.apply(logits, t, ids, float(temperature), reduction)
-    loss = _loss(rows2d(logits), t, ids, float(temperature), reduction)
+    loss = _loss(rows2d(logits), t, ids, float(temperature), reduction)[0]
     return loss.view(logits.shape[:-1]) if reduction == "none" else loss
 
 
@@ -197,11 +194,16 @@ def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: flo
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     o2 = out if out.dim() == 2 else out.detach().view(-1, out.shape[-1])
     M = l2.shape[0]
-    loss = t.new_empty(M)
-    n = _parts(t, M) if reduction == "mean" else None
-    total = None if reduction == "none" else t.new_empty(())
-    _rows(l2, t, ids, float(temperature), loss, None, None, o2, None, n, count=n is not None, total=total)
-    return (loss.view(logits.shape[:-1]) if reduction == "none" else total), out
+    if reduction == "none":
+        loss = t.new_empty(M)
+        _rows(l2, t, ids, float(temperature), loss.data_ptr(), None, None, o2)
+        return loss.view(logits.shape[:-1]), out
+    total, parts = t.new_empty(()), _parts(M) if reduction == "mean" else 0
+    own = t.new_empty(M + parts)  # the losses, then numbers of the tokens that have an entry (int32)
+    at = own.data_ptr()
+    _rows(l2, t, ids, float(temperature), at, None, None, o2, None, at + 4 * M if parts else None, parts,
+          count=1 if parts else 0, total=total.data_ptr())
+    return total, out
 
 
 class _LinearDistillFn(torch.autograd.Function):
@@ -214,11 +216,13 @@ class _LinearDistillFn(torch.autograd.Function):
         loss = torch.empty(M, device=h.device, dtype=torch.float32)
         k = t.shape[-1]
         t, ids = t.view(M, k), ids.view(M, k)
-        n = _count(t, ids, M, V)
+        n = t.new_empty(_parts(M), dtype=torch.int32)
+        launch(t, "brain_distill_count", t.data_ptr(), ids.data_ptr(), M, k, V, n.data_ptr(), n.numel())
         for s0 in range(0, M, max(chunk, 1)):
             rows = slice(s0, min(M, s0 + chunk))
             gemm(h2[rows], w, trans_b=True, out=dlogits[rows])
-            _rows(dlogits[rows], t[rows], ids[rows], temperature, loss[rows], None, None, dlogits[rows], None, n)
+            _rows(dlogits[rows], t[rows], ids[rows], temperature, loss[rows].data_ptr(), None, None, dlogits[rows], None,
+                  n.data_ptr(), n.numel())
         ctx.save_for_backward(h2, w, dlogits)
         ctx.hshape = h.shape
         total = loss.new_empty(())
