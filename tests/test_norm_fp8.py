@@ -76,7 +76,8 @@ def test_refusals():
 @pytest.mark.parametrize("shape,scaling", [
     ((1, 4096), "rowwise"), ((1, 128), "block"), ((7, 8192), "block"), ((3, 5, 768), "rowwise"), ((65, 16), "rowwise"),
     ((5, 1), "rowwise"), ((33, 1001), "rowwise"), ((2, 16384), "rowwise"), ((3, 40960), "block"), ((2, 65537), "rowwise"),
-    ((300, 384), "block"), ((129, 1024), "rowwise"), ((11, 2056), "rowwise"), ((0, 256), "rowwise")])
+    ((300, 384), "block"), ((129, 1024), "rowwise"), ((11, 2056), "rowwise"),
+    ((70, 333), "rowwise"), ((41, 7), "rowwise"), ((19, 4097), "rowwise"), ((9, 8191), "rowwise"), ((5, 12003), "rowwise"), ((0, 256), "rowwise")])
 def test_kernel(dtype, residual, shape, scaling):
     x, r, w = data(shape, dtype, 1, residual)
     args = [t.cuda() for t in (x, r, w) if t is not None]
@@ -95,6 +96,18 @@ def test_strided_and_unaligned_rows(scaling):
         xs, rs, ws = x[:, at:at + width], r[:, 1:1 + width], w[at:at + width]
         out = ops.add_rms_norm_fp8(x.cuda()[:, at:at + width], r.cuda()[:, 1:1 + width], w.cuda()[at:at + width], 1e-6, scaling)
         check(*out, xs, rs, ws, 1e-6, scaling)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width,step", [(1001, 1009), (1001, 1001 + 32), (1003, 1004), (77, 200), (5, 13)])
+def test_odd_rows_of_wider_tensors(dtype, width, step):
+    x, r, w = data((9, step), dtype, 4)
+    xs, rs, ws = x.cuda()[:, :width], r.cuda()[:, :width], w.cuda()[1:1 + width]
+    ws = ws if len(ws) == width else w.cuda()[:width]
+    out = ops.add_rms_norm_fp8(xs, rs, ws, 1e-5)
+    check(*out, xs.cpu(), rs.cpu(), ws.cpu(), 1e-5, "rowwise")
+    check(*ops.rms_norm_fp8(xs, ws, 1e-5), None, xs.cpu(), None, ws.cpu(), 1e-5, "rowwise")
 
 
 @gpu
