@@ -25,8 +25,9 @@ __device__ __forceinline__ uint8_t to_e4m3(float v) {
   return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
 }
 
-// Any width and alignment (rows that the tensors hold at different offsets, or of more than 4096 vectors): one CTA per row; a warp takes 128 values at a time, a lane every 32nd of them,
-// in the same places in all three passes, so a thread re-reads only what it wrote itself.
+// Any width and alignment (rows that the tensors hold at different offsets, or of more than 4096 vectors): one CTA
+// per row; a warp takes 128 values at a time, a lane every 32nd of them, in the same places in all three passes, so a
+// thread re-reads only what it wrote itself.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_fp8_any_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ res,
                                                            int64_t ldres, const T* __restrict__ w, T* sum_out,

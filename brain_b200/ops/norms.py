@@ -190,22 +190,22 @@ def _norm_fp8(name, x, r, w, eps, scaling):
     if not x.is_cuda:
         s = x if r is None else (x.float() + r.float()).to(x.dtype)
         return *rms_norm_fp8_ref(s, w, eps, scaling), s
-    x2 = rows2d(x)
-    M = x2.shape[0]
-    r2 = None if r is None else rows2d(r)
     w = w.contiguous()
     block = scaling == "block"
-    scale = x.new_empty((M, D // 128) if block else M, dtype=torch.float32)
-    if x2 is x and x.stride(0) == D:  # as below, without the cost of shapes
+    if len(shape) == 2 and x.is_contiguous() and (r is None or r.is_contiguous()):  # as below, at less cost a call
+        x2, r2, M, ldx, ldr = x, r, shape[0], D, D
         q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
         s = None if r is None else torch.empty_like(x)
     else:
-        q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
-        s = None if r is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        if x.dim() != 2:
-            scale = scale.view(*x.shape[:-1], D // 128) if block else scale.view(x.shape[:-1])
-    launch(x, "brain_norm_fp8", code, x2.data_ptr(), x2.stride(0), ptr(r2), 0 if r2 is None else r2.stride(0),
-           w.data_ptr(), ptr(s), q.data_ptr(), scale.data_ptr(), M, D, int(block), float(eps))
+        x2, r2 = rows2d(x), None if r is None else rows2d(r)
+        M, ldx, ldr = x2.shape[0], x2.stride(0), 0 if r2 is None else r2.stride(0)
+        q = torch.empty(shape, device=x.device, dtype=torch.float8_e4m3fn)
+        s = None if r is None else torch.empty(shape, device=x.device, dtype=x.dtype)
+    scale = x.new_empty((M, D // 128) if block else M, dtype=torch.float32)
+    if len(shape) != 2:
+        scale = scale.view(*shape[:-1], D // 128) if block else scale.view(shape[:-1])
+    launch(x, "brain_norm_fp8", code, x2.data_ptr(), ldx, ptr(r2), ldr, w.data_ptr(), ptr(s), q.data_ptr(),
+           scale.data_ptr(), M, D, int(block), float(eps))
     return q, scale, s
 
 
