@@ -167,11 +167,25 @@ def _apart(out, logits):
     return lo + span * size <= lo2 or lo2 + other * size <= lo
 
 
+def _plain(out):
+    """``out`` for the caller, without the history that it may have as logits."""
+    return out.detach() if out.requires_grad else out
+
+
+def _written(out, given):
+    """What was written by address into a caller's tensor is told to autograd: a graph that saved its values raises in
+    its backward pass, as after any write in place."""
+    if given and not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return _plain(out)
+
+
 def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: float = 1.0, reduction: str = "mean",
                            out: torch.Tensor | None = None):
     """(loss, dloss/dlogits) of :func:`topk_distillation` (with ``"none"`` the gradient of the losses' sum),
     outside autograd. ``out`` takes the gradient: of logits' shape and type with adjacent columns, or logits
-    itself."""
+    itself, whose own history stays (``logits.backward(grad)``); autograd sees the write, so a graph that saved the
+    values of ``out`` raises in its backward pass."""
     name = "topk_distillation_grad"
     _check(name, logits, teacher_logits, teacher_ids, temperature, reduction)
     if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.stride(-1) != 1):
@@ -184,26 +198,29 @@ def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: flo
             z = logits.detach().requires_grad_()
             loss = topk_distillation_ref(z, teacher_logits, teacher_ids, temperature, reduction)
             grad = torch.autograd.grad(loss.sum(), z)[0]
-        return loss.detach(), grad if out is None else out.copy_(grad)
+        if out is not None:
+            out.detach().copy_(grad)
+        return loss.detach(), grad if out is None else _plain(out)
     dtype_code(name, logits)
     if logits.requires_grad:
         logits = logits.detach()
     t, ids = _teacher(teacher_logits, teacher_ids)
     l2 = rows2d(logits)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     o2 = out if out.dim() == 2 else out.detach().view(-1, out.shape[-1])
     M = l2.shape[0]
     if reduction == "none":
         loss = t.new_empty(M)
         _rows(l2, t, ids, float(temperature), loss.data_ptr(), None, None, o2)
-        return loss.view(logits.shape[:-1]), out
+        return loss.view(logits.shape[:-1]), _written(out, given)
     total, parts = t.new_empty(()), _parts(M) if reduction == "mean" else 0
     own = t.new_empty(M + parts)  # the losses, then numbers of the tokens that have an entry (int32)
     at = own.data_ptr()
     _rows(l2, t, ids, float(temperature), at, None, None, o2, None, at + 4 * M if parts else None, parts,
           count=1 if parts else 0, total=total.data_ptr())
-    return total, out
+    return total, _written(out, given)
 
 
 class _LinearDistillFn(torch.autograd.Function):

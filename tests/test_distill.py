@@ -164,6 +164,41 @@ def test_refusals():
         ops.linear_topk_distillation(torch.randn(3, 8), torch.randn(20, 9), t, ids)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_gradient_in_place_of_logits_with_a_history(device, reduction):
+    dtype = torch.float32
+    _, t, ids = (x.to(device) for x in data(6, 40, 5, dtype, 12))
+    g = torch.Generator().manual_seed(13)
+    h, w = torch.randn(6, 8, generator=g).to(device), torch.randn(40, 8, generator=g).to(device).requires_grad_()
+    grads = []
+    for there in (False, True):
+        z = h @ w.t()
+        before = z.detach().clone()
+        loss, grad = ops.topk_distillation_grad(z, t, ids, 1.5, reduction, out=z if there else None)
+        assert not loss.requires_grad and not grad.requires_grad
+        assert (z.data_ptr() == grad.data_ptr()) == there and (there or torch.equal(z, before))
+        z.backward(grad)
+        grads.append(w.grad)
+        w.grad = None
+    assert (grads[0] != 0).any() and torch.equal(*grads)
+    # what was saved before the write is no longer there (on the CPU the loss saves none of it)
+    z = h @ w.t()
+    pending, square = ops.topk_distillation(z, t, ids, 1.5), z * z
+    kept = torch.tanh(z)
+    ops.topk_distillation_grad(z, t, ids, 1.5, reduction, out=z)
+    for saved in (square.sum(), pending)[:1 if device == "cpu" else 2]:
+        with pytest.raises(RuntimeError):
+            saved.backward()
+    ops.topk_distillation_grad(h @ w.t(), t, ids, 1.5, reduction, out=kept)
+    with pytest.raises(RuntimeError):
+        kept.sum().backward()
+    leaf = z.detach().requires_grad_()
+    want = ops.topk_distillation_grad(leaf, t, ids, 1.5, reduction)[1]
+    grad = ops.topk_distillation_grad(leaf, t, ids, 1.5, reduction, out=leaf)[1]
+    assert torch.equal(grad, want) and leaf.requires_grad and leaf.is_leaf
+
+
 # ------------------------------------------------------------------ kernels
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
