@@ -194,8 +194,8 @@ def topk_distillation_grad(logits, teacher_logits, teacher_ids, temperature: flo
     if out is not None and not _apart(out, logits):
         raise ValueError(f"{name}: out shares memory with itself or with logits without being logits")
     if not logits.is_cuda:
-        with torch.enable_grad():
-            z = logits.detach().requires_grad_()
+        with torch.inference_mode(False), torch.enable_grad():
+            z = (logits.clone() if logits.is_inference() else logits).detach().requires_grad_()
             loss = topk_distillation_ref(z, teacher_logits, teacher_ids, temperature, reduction)
             grad = torch.autograd.grad(loss.sum(), z)[0]
         if out is not None:

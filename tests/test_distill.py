@@ -199,6 +199,18 @@ def test_gradient_in_place_of_logits_with_a_history(device, reduction):
     assert torch.equal(grad, want) and leaf.requires_grad and leaf.is_leaf
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_gradient_under_inference_mode(device):
+    z, t, ids = (x.to(device) for x in data(6, 40, 5, torch.float32, 14))
+    want = ops.topk_distillation_grad(z, t, ids, 1.5)
+    with torch.inference_mode():
+        for args in ((z, t, ids), (z.clone(), t.clone(), ids.clone())):
+            got = ops.topk_distillation_grad(*args, 1.5)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        there = z.clone()
+        assert ops.topk_distillation_grad(there, t, ids, 1.5, out=there)[1] is there and torch.equal(there, want[1])
+
+
 # ------------------------------------------------------------------ kernels
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
