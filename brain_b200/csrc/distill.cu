@@ -516,7 +516,8 @@ int launch(const DistillArgs& a, int64_t M, cudaStream_t st) {
     return (int)cudaGetLastError();
   }
   const auto run = [&](auto kernel, int threads, int ring) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring + smem);
+    // one limit for every k: it belongs to the kernel, and another thread's call may set it before this one's launch
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring + kMaxTop * 12);
     if (e != cudaSuccess) return (int)e;
     kernel<<<(unsigned)M, threads, ring + smem, st>>>(a);
     return (int)cudaGetLastError();

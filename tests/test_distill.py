@@ -1,10 +1,11 @@
 """Distillation from a teacher's kept logits: loss and gradient against the formula in 64 bits and differences."""
 import math
+import threading
 
 import pytest
 import torch
 
-from brain_b200 import losses, ops
+from brain_b200 import _native, losses, ops
 from brain_b200.models import LlamaLite, LlamaLiteConfig
 
 gpu = pytest.mark.gpu
@@ -349,6 +350,39 @@ def test_two_graphs_of_the_same_leaf_and_repeated_backward():
     graph.replay()
     assert torch.equal(auto, want)
     assert torch.equal(got, ops.topk_distillation_grad(leaf.detach(), t, ids, 2.0)[1])
+
+
+@gpu
+@pytest.mark.parametrize("rows,V", [(1, 120000), (160, 25000)])
+def test_calls_of_several_threads(rows, V):
+    """Few and many kept entries at once, on streams of their own: each call gets the shared memory that it needs. The
+    entry point itself is called, as the host time around it would keep the threads apart."""
+    call, kept = _native.fn("brain_distill_rows"), (1024, 1, 1024, 1)
+    cases = [tuple(x.cuda() for x in data(rows, V, k, torch.float32, k)) for k in kept]
+    want = [ops.topk_distillation(*c, 2.0, "none") for c in cases]
+    losses, streams = [torch.zeros(rows, device="cuda") for _ in kept], [torch.cuda.Stream() for _ in kept]
+    torch.cuda.synchronize()
+    gate, failed = threading.Barrier(len(kept)), []
+
+    def calls(i):
+        z, t, ids = cases[i]
+        gate.wait()
+        for j in range(3000):
+            rc = call(2, z.data_ptr(), V, t.data_ptr(), ids.data_ptr(), losses[i].data_ptr(), None, None, None, 0, None,
+                      None, 0, 0, 0, rows, kept[i], V, 2.0, None, streams[i].cuda_stream)
+            if rc:
+                failed.append((kept[i], j, rc))
+            if j % 200 == 199:
+                streams[i].synchronize()
+
+    threads = [threading.Thread(target=calls, args=(i,)) for i in range(len(kept))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    assert all(torch.equal(a, b) for a, b in zip(losses, want))
 
 
 @gpu
