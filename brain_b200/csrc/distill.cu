@@ -43,7 +43,7 @@ struct DistillArgs {
   float* counts;         // [M], 1 where the row has an entry, else 0; may be null
   void* dz;              // null for the loss alone
   int64_t lddz;
-  const float* grad;     // upstream gradient: a scalar, or one a row
+  const float* grad;     // upstream gradient of the backward pass: a scalar, or one a row
   const int* n;          // numbers of rows that count, to be added up and divided by; null: no division
   int parts;             // how many
   int grad_rows;
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kStream) distill_grad_kernel(DistillArgs a, in
   sum = block_sum_all(sum, red);
   const float factor = a.inv_t * kLog2e, lse2 = a.lse[row] * kLog2e;
   const float by = inv_count(a.n, a.parts);
-  const float g = any ? (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * by * a.temp : 0.f;
+  const float g = any ? a.grad[a.grad_rows ? row : 0] * by * a.temp : 0.f;
   for (int at = sl.v0; at < sl.v1; at += U * kStream) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -411,18 +411,17 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
   }
   if (!GRAD) return;
 
-  // ---- the gradient: g 2^x is 2^(x + log2 |g|), with its sign set afterwards
+  // ---- the gradient: g 2^x is 2^(x + log2 g)
   T* dz = (T*)a.dz + row * a.lddz;
   const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
-  const float g = (a.grad ? a.grad[a.grad_rows ? row : 0] : 1.f) * by * a.temp;
+  const float g = by * a.temp;
   if (!any) {  // zeros, also where logits are infinite or NaN
     for (int i = tid; i < sl.nv; i += kRow) put(dz, sl.head + i * W::N, make_uint4(0, 0, 0, 0), alike);
     if (end >= 0) dz[end] = from_f32<T>(0.f);
     return;
   }
-  const float lse2 = lse * kLog2e, shift = log2f(fabsf(g)) - lse2;
+  const float lse2 = lse * kLog2e, shift = log2f(g) - lse2;
   const uint64_t shift2 = two(shift, shift);
-  const uint32_t sign = g < 0.f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
   // what the ring holds first (its oldest block is in `slot`), then the others from the row's start
   const int kept = min(S, blocks);
   if (blocks < S) slot = 0;
@@ -442,8 +441,8 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
         if (W::PER == 1) f[1] = __uint_as_float(word(v, e4 + (W::PER == 1)));
         one_each(fma2(two(f[0], f[1]), factor2, shift2), f[0], f[1]);
         f[0] = ex2(f[0]), f[1] = ex2(f[1]);
-        set_word(o, e4, W::pack(f) ^ sign);
-        if (W::PER == 1) set_word(o, e4 + (W::PER == 1), W::pack(f + 1) ^ sign);
+        set_word(o, e4, W::pack(f));
+        if (W::PER == 1) set_word(o, e4 + (W::PER == 1), W::pack(f + 1));
       }
       put(dz, sl.head + i * W::N, o, alike);
     }
@@ -556,16 +555,16 @@ BRAIN_API int brain_distill_reduce(const float* loss, const float* counts, int64
   return (int)cudaGetLastError();
 }
 
-// Rows: loss [M] (null: take lse), lse [M] (may be null with loss), counts [M] (may be null), dz (null: none; may
-// be z) with its row stride. The gradient is scaled by grad (null: 1; one a row with
-// grad_rows) and divided by the sum of n's parts (null: no division), which are counted first with `count`. Where total
+// Rows: loss [M] (null in the backward pass, which takes lse and the upstream gradient grad, one a row with grad_rows),
+// lse [M] (may be null with loss), counts [M] (may be null), dz (null: none; may be z) with its row stride. The gradient
+// is divided by the sum of n's parts (null: no division), which are counted first with `count`. Where total
 // is given, brain_distill_reduce follows (all in one call, as a call from Python costs as much as a small kernel).
 BRAIN_API int brain_distill_rows(int dtype, const void* z, int64_t ldz, const float* t, const int64_t* id, float* loss,
                                  float* lse, float* counts, void* dz, int64_t lddz, const float* grad, int* n,
                                  int parts, int count, int grad_rows, int64_t M, int k, int V, float temp, float* total,
                                  cudaStream_t st) {
   if (M < 0 || V <= 0 || V > (1 << 30) || k <= 0 || k > kMaxTop || M > INT32_MAX || !(temp > 0.f) ||
-      (M > 0 && !loss && (!dz || !lse || total)))
+      (M > 0 && (loss ? grad || grad_rows : !dz || !lse || !grad || total)))
     return (int)cudaErrorInvalidValue;
   if (count) {
     const int e = brain_distill_count(t, id, M, k, V, n, parts, st);

@@ -212,6 +212,18 @@ def test_gradient_under_inference_mode(device):
         assert ops.topk_distillation_grad(there, t, ids, 1.5, out=there)[1] is there and torch.equal(there, want[1])
 
 
+def test_refusals_of_the_entry_point():
+    """Before anything is launched: an upstream gradient belongs to the backward pass, which needs it and the row's
+    log-sum-exp; sizes and temperatures out of range. The addresses are never used."""
+    def call(loss=16, lse=16, dz=16, grad=None, grad_rows=0, M=1, k=1, V=8, T=1.0, total=None):
+        return _native.fn("brain_distill_rows")(2, 16, V, 16, 16, loss, lse, None, dz, V, grad, None, 0, 0, grad_rows, M, k, V,
+                                                T, total, None)
+    for bad in (dict(grad=16), dict(grad_rows=1), dict(loss=None), dict(loss=None, grad=16, lse=None),
+                dict(loss=None, grad=16, dz=None), dict(loss=None, grad=16, total=16), dict(k=0), dict(k=1025), dict(V=0),
+                dict(V=2 ** 30 + 1), dict(M=-1), dict(M=2 ** 31), dict(T=0.0)):
+        assert call(**bad) == 1, bad  # cudaErrorInvalidValue
+
+
 # ------------------------------------------------------------------ kernels
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
