@@ -5,7 +5,7 @@
 //   token i is accepted while u_i q_i(x_i) < p_i(x_i); n = the first refused i, or L;
 //   the next token is drawn from r = max(p_n - q_n, 0) (from p_n when r is empty, and when n == L) by
 //   inversion: the smallest j with r_0 + .. + r_j > u_K (r_0 + .. + r_{V-1}).
-// Weights that are negative, infinite or NaN weigh nothing. The emitted tokens are distributed as the
+// Probabilities that are negative, infinite or NaN count as 0 throughout. The emitted tokens are distributed as the
 // target's own samples are.
 //
 // The ids have to be the same however the sums are split, so products and sums are held in 64 bits: the
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(VerifyArgs a) {
         const int64_t x = drafted[i];
         refused = true;
         if (x >= 0 && x < a.V) {
-          const double pi = to_f32(pb[i * a.p_pos + x]), qi = qb ? to_f32(qb[i * a.q_pos + x]) : 1.f;
+          const double pi = weight(to_f32(pb[i * a.p_pos + x])), qi = qb ? weight(to_f32(qb[i * a.q_pos + x])) : 1.f;
           refused = !((double)u[i] * qi < pi);
         }
       }

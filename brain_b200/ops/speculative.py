@@ -19,8 +19,9 @@ def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_l
     Token i is accepted while ``uniforms[i] * q_i < p_i``. Row b of ``tokens`` holds the accepted tokens, then
     one drawn from max(p - q, 0) at the first refusal (from p where that is empty, or where nothing was
     refused) as the first id whose running sum exceeds ``uniforms[b, K]`` times the whole, then -1. Sums are
-    taken in 64 bits. Probabilities need not sum to one; negative, infinite and NaN ones weigh nothing, a
-    drafted id outside the vocabulary is refused, and a row without any weight gives token -1."""
+    taken in 64 bits. Probabilities need not sum to one; negative, infinite and NaN ones count as 0 throughout (so a
+    token without any probability of the target's is refused, whatever the draft's), a drafted id outside the
+    vocabulary is refused, and a row without any weight gives token -1."""
     if target_probs.dim() != 3 or draft_tokens.dim() != 2:
         raise ValueError("verify_draft takes target_probs [B, K + 1, V] and draft_tokens [B, K]")
     B, K1, V = target_probs.shape
@@ -79,8 +80,8 @@ def verify_draft_ref(target_probs, draft_tokens, uniforms, draft_probs=None, dra
             x = int(draft_tokens[b, n])
             if not 0 <= x < V:
                 break
-            q = 1.0 if draft_probs is None else float(draft_probs[b, n, x])
-            if not float(u[b, n]) * q < float(target_probs[b, n, x]):
+            q = 1.0 if draft_probs is None else float(weights(draft_probs[b, n, x]))
+            if not float(u[b, n]) * q < float(weights(target_probs[b, n, x])):
                 break
             tokens[b, n] = x
             n += 1

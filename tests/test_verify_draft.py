@@ -39,6 +39,24 @@ def test_definition_by_hand():
     assert tokens.tolist() == [[1, -1, -1]] and n.tolist() == [0]
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("p0,q0,kept", [(INF, 0.5, False), (NAN, 0.5, False), (-0.5, 0.5, False), (0.0, -0.5, False),
+                                        (0.0, INF, False), (0.0, NAN, False), (0.5, NAN, True), (0.5, INF, True),
+                                        (0.5, -0.5, True), (0.5, 0.0, True), (-0.25, -0.5, False), (INF, NAN, False)])
+@pytest.mark.parametrize("u", [0.0, 0.5])
+def test_acceptance_of_weights_that_are_none(device, p0, q0, kept, u):
+    """A drafted id whose probability is negative, infinite or NaN on either side: 0 there, as in the sums. A refused
+    one is followed by id 1, all that is left, an accepted one by id 2."""
+    p = torch.tensor([[[p0, 0.5, 0.0], [0.0, 0.0, 1.0]]], device=device)
+    q = torch.tensor([[[q0, 0.25, 0.0]]], device=device)
+    x, us = torch.tensor([[0]], device=device), torch.tensor([[u, 0.5]], device=device)
+    tokens, n = ops.verify_draft(p, x, us, q)
+    assert tokens.tolist() == ([[0, 2]] if kept else [[1, -1]]) and n.tolist() == [int(kept)]
+    if q0 == 0.5 and kept is False:  # a certain draft
+        tokens, n = ops.verify_draft(p, x, us)
+        assert tokens.tolist() == [[1, -1]] and n.tolist() == [0]
+
+
 def test_samples_are_the_targets():
     """Over many draws the emitted first token has the target's probabilities."""
     g = torch.Generator().manual_seed(3)
