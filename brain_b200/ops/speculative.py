@@ -52,7 +52,7 @@ def verify_draft(target_probs, draft_tokens, uniforms, draft_probs=None, draft_l
     drafted = drafted.contiguous()
     lens = draft_lens
     if lens is not None:
-        lens = (lens if lens.dtype == torch.int32 else lens.clamp(0, K).int()).contiguous()
+        lens = (lens if lens.dtype == torch.int32 else lens.long().clamp(0, K).int()).contiguous()
     u = uniforms.contiguous()
     tokens = drafted.new_empty((B, K1))
     count = drafted.new_empty(B)

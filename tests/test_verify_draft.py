@@ -156,6 +156,19 @@ def test_strides_and_index_types():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.int64])
+def test_lengths_of_any_whole_type(dtype):
+    """More drafted tokens than the lengths' own type counts."""
+    K = 40000 if dtype in (torch.int16, torch.uint16) else 300
+    p = torch.full((3, 1, 4), 0.25, device="cuda").expand(3, K + 1, 4)
+    x = torch.zeros(3, K, dtype=torch.long, device="cuda")
+    u = torch.zeros(3, K + 1, device="cuda")
+    lens = torch.tensor([0, 3, 100]).to(dtype)
+    tokens, n = ops.verify_draft(p, x, u, None, lens.cuda())
+    assert n.tolist() == [0, 3, 100] and (tokens >= 0).sum(1).tolist() == [1, 4, 101]
+
+
+@gpu
 def test_rows_beyond_32_bit_offsets():
     """The last sequence starts more than 2^31 values into the target's probabilities."""
     V, B = 128256, 2100
