@@ -145,7 +145,7 @@ def main_grad_beta(p: torch.Tensor) -> float:
 
 def rows2d(x: torch.Tensor) -> torch.Tensor:
     """View x as [rows, last] with unit last-dim stride (copying only if needed)."""
-    if x.dim() == 2 and x.stride(1) == 1:
+    if x.dim() == 2 and x.stride(1) == 1 and x.shape[1] > 0:  # reshape refuses rows without values
         return x
     x2 = x.reshape(-1, x.shape[-1])
     if x2.stride(-1) != 1:
