@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -98,12 +99,21 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: _native.stream_ptr(torch.device("cuda", index)))
 
 
+def has_tangent(t: torch.Tensor) -> bool:
+    """Whether forward-mode differentiation follows ``t``. What a kernel makes of its address would lose that."""
+    # without a level there is none, and unpacking costs 0.7 us
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def no_backward(name: str, *tensors) -> None:
-    """Raise when autograd would record an inference op: its result would carry no gradient, silently."""
+    """Raise when autograd, backward or forward, would record an inference op: its result would carry no derivative,
+    silently."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0 and any(t is not None and has_tangent(t) for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative: call it on unpacked tensors")
 
 
 def stream(t: torch.Tensor) -> int:

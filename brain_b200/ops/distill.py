@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._common import DTYPE_CODES, dtype_code, has_main_grad, launch, main_grad_beta, ptr, rows2d, same_device
+from ._common import DTYPE_CODES, dtype_code, has_main_grad, has_tangent, launch, main_grad_beta, ptr, rows2d, same_device
 from .gemm import gemm
 
 MAX_TOP = 1024
@@ -43,7 +43,7 @@ def _check(name, logits, teacher_logits, teacher_ids, temperature, reduction):
         raise TypeError(f"{name}: teacher_ids are whole numbers")
     if teacher_logits.dtype is not torch.float32 and not teacher_logits.is_floating_point():
         raise TypeError(f"{name}: teacher_logits are floating-point numbers")
-    if teacher_logits.requires_grad and torch.is_grad_enabled():
+    if teacher_logits.requires_grad and torch.is_grad_enabled() or has_tangent(teacher_logits):
         raise RuntimeError(f"{name} gives the teacher no gradient: detach teacher_logits")
     same_device(logits, teacher_logits, teacher_ids)
 
@@ -145,7 +145,7 @@ def topk_distillation(logits, teacher_logits, teacher_ids, temperature: float = 
         return topk_distillation_ref(logits, teacher_logits, teacher_ids, temperature, reduction)
     dtype_code("topk_distillation", logits)
     t, ids = _teacher(teacher_logits, teacher_ids)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if torch.is_grad_enabled() and logits.requires_grad or has_tangent(logits):  # which raises for the latter
         return _DistillFn.apply(logits, t, ids, float(temperature), reduction)
     loss = _loss(rows2d(logits), t, ids, float(temperature), reduction)[0]
     return loss.view(logits.shape[:-1]) if reduction == "none" else loss

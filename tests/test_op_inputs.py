@@ -1,8 +1,10 @@
 """What the ops' shared helpers refuse and count, whichever op calls them."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from brain_b200 import ops
+from brain_b200 import quantization as Q
 from brain_b200.ops._common import rows2d
 
 gpu = pytest.mark.gpu
@@ -30,3 +32,33 @@ def test_rows_of_a_tensor(shape, rows):
 def test_ops_refuse_rows_without_values(call):
     with pytest.raises((RuntimeError, ValueError)):
         call(torch.empty(3, 0, device="cuda", dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_is_followed_or_refused(device, grad_mode):
+    """A dual tensor that asks for no gradient: its tangent must not get lost, with or without a backward pass."""
+    g = torch.Generator().manual_seed(0)
+    x, z = (torch.randn(4, 128, generator=g).to(device) for _ in range(2))
+    t, ids = torch.randn(4, 3, generator=g).to(device), torch.tensor([[0, 1, 5]] * 4, device=device)
+    packed, scales, _ = Q.quantize_int4(torch.randn(8, 128, generator=g), 64)
+    packed, scales = packed.to(device), scales.to(device)
+    w = torch.ones(128, device=device)
+    with fwd.dual_level(), torch.set_grad_enabled(grad_mode):
+        d, half = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(x.bfloat16(), torch.ones_like(x).bfloat16())
+        for call in (lambda: ops.rms_norm_fp8(d, w), lambda: ops.add_rms_norm_fp8(x, d, w),
+                     lambda: ops.rms_norm_fp8(x, fwd.make_dual(w, w)), lambda: Q.int4_linear(half, packed, scales, group_size=64),
+                     lambda: ops.topk_distillation(z, fwd.make_dual(t, t), ids)):
+            with pytest.raises(RuntimeError):
+                call()
+        if device == "cuda":
+            with pytest.raises(NotImplementedError):
+                ops.topk_distillation(d, t, ids)
+        else:
+            h = 1e-3
+            slope = fwd.unpack_dual(ops.topk_distillation(d * d, t, ids, 1.5)).tangent
+            hi, lo = (ops.topk_distillation((x.double() + s * h) ** 2, t, ids, 1.5) for s in (1, -1))
+            # differences are off by h^2 times a third derivative of order 100, f32 by a few 2^-24 of it
+            assert abs(float(slope - (hi - lo) / (2 * h))) < 1e-3
+        # tensors without a tangent are taken as before
+        ops.rms_norm_fp8(x, w), Q.int4_linear(x.bfloat16(), packed, scales, group_size=64), ops.topk_distillation(z, t, ids)
