@@ -97,12 +97,18 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-# Kernels launched by one call of each multi-kernel entry point (default 1); used to count this
-# library's launches inside a timed region (``launch_counter``).
+# Kernels launched by one call of each multi-kernel entry point (default 1), or a function of its arguments;
+# used to count this library's launches inside a timed region (``launch_counter``).
 KERNELS_PER_CALL = {
     "brain_norm_bwd": 2, "brain_attn_bwd": 4, "brain_sumsq": 2, "brain_error_string": 0,
     "brain_norm_bwd_partials": 0, "brain_gemm_splitk_plan": 0, "brain_gemm_bf16_ws": 2,
     "brain_colsum_partials": 0, "brain_colsum_bf16": 2,
+    # the count, the rows (none of none), the sum
+    "brain_distill_rows": lambda a: bool(a[13]) + (a[15] > 0) + (a[19] is not None),
+    # one for 32768 inputs
+    "brain_int4_linear": lambda a: -(-a[12] // 32768) if a[10] > 0 and a[11] > 0 else 0,
+    "brain_norm_fp8": lambda a: int(a[9] > 0),
+    "brain_verify_draft": lambda a: int(a[12] > 0),
 }
 _launches = {"on": False, "n": 0}
 
@@ -133,7 +139,8 @@ def set_nvtx(on: bool) -> None:
 
 def call(name: str, *args) -> int:
     if _launches["on"]:
-        _launches["n"] += KERNELS_PER_CALL.get(name, 1)
+        n = KERNELS_PER_CALL.get(name, 1)
+        _launches["n"] += n(args) if callable(n) else n
     if _nvtx["on"]:
         torch.cuda.nvtx.range_push(name)
         try:

@@ -3,7 +3,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from brain_b200 import ops
+from brain_b200 import _native, ops
 from brain_b200 import quantization as Q
 from brain_b200.ops._common import rows2d
 
@@ -62,3 +62,34 @@ def test_forward_mode_is_followed_or_refused(device, grad_mode):
             assert abs(float(slope - (hi - lo) / (2 * h))) < 1e-3
         # tensors without a tangent are taken as before
         ops.rms_norm_fp8(x, w), Q.int4_linear(x.bfloat16(), packed, scales, group_size=64), ops.topk_distillation(z, t, ids)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [0, 3])
+def test_launches_are_counted(rows):
+    """Each operator's kernels, by what its call asks for."""
+    some = int(rows > 0)
+    z, t = (torch.zeros(rows, n, device="cuda", requires_grad=n == 64) for n in (64, 2))
+    ids = torch.zeros(rows, 2, device="cuda", dtype=torch.long)
+    flat = z.detach()
+    h, w = (torch.zeros(n, 64, device="cuda", dtype=torch.bfloat16) for n in (rows, 64))
+    x = torch.zeros(rows, 40960, device="cuda", dtype=torch.bfloat16)
+    packed, scales = torch.zeros(4, 20480, device="cuda", dtype=torch.uint8), torch.ones(4, 320, device="cuda").bfloat16()
+    p, ones = torch.ones(rows, 3, 8, device="cuda"), torch.ones(64, device="cuda")
+    for call, kernels in (
+            (lambda: ops.topk_distillation(flat, t, ids, reduction="none"), some),
+            (lambda: ops.topk_distillation(flat, t, ids), some + 1),
+            (lambda: ops.topk_distillation(z, t, ids).backward(), 2 * some + 1),
+            (lambda: ops.topk_distillation_grad(flat, t, ids, reduction="none"), some),
+            (lambda: ops.topk_distillation_grad(flat, t, ids, reduction="sum"), some + 1),
+            (lambda: ops.topk_distillation_grad(flat, t, ids), some + 2),
+            (lambda: ops.linear_topk_distillation(h, w, t, ids), 2 * some + 2),
+            (lambda: ops.linear_topk_distillation(h, w, t, ids, chunk=1), 2 * rows + 2),
+            (lambda: Q.int4_linear(x, packed, scales), 2 * some),
+            (lambda: Q.int4_linear(x[:, :1024], packed[:, :512].contiguous(), scales[:, :8]), some),
+            (lambda: ops.rms_norm_fp8(flat, ones), some),
+            (lambda: ops.verify_draft(p, ids, p[..., 0]), some)):
+        with _native.launch_counter() as counter:
+            call()
+        assert counter.count == kernels
+    torch.cuda.synchronize()
