@@ -276,4 +276,5 @@ def linear_topk_distillation(h, w, teacher_logits, teacher_ids, temperature: flo
     for x in (h, w):
         dtype_code("linear_topk_distillation", x, (torch.bfloat16,))
     t, ids = _teacher(teacher_logits, teacher_ids)
-    return _LinearDistillFn.apply(h, w, t, ids, float(temperature), chunk)
+    with torch.cuda.device(h.device):  # the GEMM launches on the current one
+        return _LinearDistillFn.apply(h, w, t, ids, float(temperature), chunk)

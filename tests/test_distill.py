@@ -422,6 +422,34 @@ def test_linear(V, chunk, main):
 
 
 @gpu
+@pytest.mark.multigpu
+def test_tensors_of_another_device_than_the_current_one():
+    z, t, ids = data(40, 64, 4, torch.float32, 15)
+    h, w = (torch.randn(n, 32, generator=torch.Generator().manual_seed(n)).bfloat16() for n in (40, 64))
+    got = []
+    for device in ("cuda:0", "cuda:1"):
+        with torch.cuda.device(0):
+            tc, ic = t.to(device), ids.to(device)
+            loss, grad = ops.topk_distillation_grad(z.to(device), tc, ic)
+            hd, wd = h.to(device).requires_grad_(), w.to(device).requires_grad_()
+            head = ops.linear_topk_distillation(hd, wd, tc, ic)
+            head.backward()
+            got.append([x.cpu() for x in (loss, grad, head, hd.grad, wd.grad)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@gpu
+@pytest.mark.parametrize("chunk", [0, 4])
+def test_linear_without_tokens(chunk):
+    h = torch.zeros(2, 0, 32, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.randn(64, 32, device="cuda").bfloat16().requires_grad_()
+    loss = ops.linear_topk_distillation(h, w, torch.zeros(2, 0, 3, device="cuda"), torch.zeros(2, 0, 3, device="cuda").long(),
+                                        chunk=chunk)
+    loss.backward()
+    assert loss.item() == 0 and h.grad.shape == h.shape and (w.grad == 0).all()
+
+
+@gpu
 def test_a_language_model_learns_from_it():
     cfg = LlamaLiteConfig(vocab_size=256, hidden_dim=128, num_layers=1, num_heads=2, num_kv_heads=2, head_dim=64,
                           intermediate_dim=256, max_seq_len=64)
