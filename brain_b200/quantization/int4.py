@@ -27,11 +27,21 @@ def _check_group(K: int, group_size: int) -> None:
         raise ValueError(f"group size {group_size} does not divide {_SLAB}, as more inputs than that need it to")
 
 
+def _scale(wanted: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Group scales in their type. Its subnormals are far apart (f16's begin at 6e-5, where small weights lie), so these
+    round up: a scale rounded down by up to half would cut the largest values off. f32's own are not used."""
+    info = torch.finfo(dtype)
+    least = max(info.tiny * info.eps, 2.0 ** -126)
+    up = torch.ceil(wanted / least).clamp_min(1) * least
+    return torch.where(wanted < info.tiny, up, wanted).to(dtype)
+
+
 def quantize_int4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True,
                   scale_dtype: torch.dtype = torch.bfloat16):
     """w [N, K] -> (packed [N, K / 2] uint8, scales [N, groups], zeros [N, groups] uint8 or None). The scale is
     max |w| / 7 of its group, or (max - min) / 15 with zero points (of a range that holds 0), rounded to
-    ``scale_dtype`` before the values are; the last group of a K that ``group_size`` does not divide is shorter."""
+    ``scale_dtype`` before the values are (up, where it is subnormal there; at least 2^-126 and what the type can hold); the
+    last group of a K that ``group_size`` does not divide is shorter."""
     if w.dim() != 2:
         raise ValueError(f"quantize_int4 takes a [N, K] weight, not {tuple(w.shape)}")
     N, K = w.shape
@@ -40,14 +50,13 @@ def quantize_int4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True
         raise TypeError(f"quantize_int4: scales are bfloat16 or float16, not {scale_dtype}")
     groups = -(-K // group_size)
     x = torch.nn.functional.pad(w.detach().float(), (0, groups * group_size - K)).view(N, groups, group_size)
-    tiny = torch.finfo(scale_dtype).tiny
     if symmetric:
-        scales = (x.abs().amax(-1) / 7).clamp_min(tiny).to(scale_dtype)
+        scales = _scale(x.abs().amax(-1) / 7, scale_dtype)
         q = torch.round(x / scales.float()[..., None]).clamp(-8, 7)
         zeros = None
     else:
         lo, hi = x.amin(-1).clamp_max(0), x.amax(-1).clamp_min(0)
-        scales = ((hi - lo) / 15).clamp_min(tiny).to(scale_dtype)
+        scales = _scale((hi - lo) / 15, scale_dtype)
         z = torch.round(-lo / scales.float()).clamp(0, 15)
         q = torch.round(x / scales.float()[..., None] + z[..., None]).clamp(0, 15)
         zeros = z.to(torch.uint8)

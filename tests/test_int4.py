@@ -58,6 +58,39 @@ def test_quantiser(symmetric, K, G):
         assert torch.equal(flat.view(9, -1), packed)  # the byte order of pack_int4
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [1.0, 1e-4, 3e-6, 2.0 ** -24, 1e-9, 0.0])
+def test_scales_of_small_weights(device, symmetric, dtype, size):
+    """No value is further from its weight than half a step, of a scale that is no larger than the group asks for and the
+    type lets it be."""
+    w = torch.randn(5, 256, generator=torch.Generator().manual_seed(3)) * size
+    packed, scales, zeros = Q.quantize_int4(w.to(device), 64, symmetric, dtype)
+    assert scales.dtype == dtype and (scales > 0).all() and torch.isfinite(scales).all()
+    cut = w.view(5, 4, 64).double()
+    lo, hi = cut.amin(-1).clamp_max(0), cut.amax(-1).clamp_min(0)
+    wanted = cut.abs().amax(-1) / 7 if symmetric else (hi - lo) / 15
+    info = torch.finfo(dtype)
+    got, least = scales.cpu().double(), max(info.tiny * info.eps, 2.0 ** -126)
+    # normal scales round by half a step, subnormal ones up by less than one; f32 on the way adds 2^-23
+    assert (got <= wanted * (1 + info.eps / 2 + 2.0 ** -23) + least).all()
+    assert (got >= wanted * (1 - info.eps / 2 - 2.0 ** -23)).all()
+    back = Q.dequantize_int4(packed, scales, zeros, 64).cpu().double().view_as(cut)
+    # as in test_quantiser: what a scale rounded down leaves out at the ends, and a rounded zero point
+    far = 0.5 + 15 * (info.eps / 2 + 2.0 ** -22) + (0 if symmetric else 0.5)
+    assert ((back - cut).abs() <= far * got[..., None]).all()
+
+
+def test_small_weights_keep_their_levels_in_f16():
+    w = torch.randn(64, 1024, generator=torch.Generator().manual_seed(4))
+    for symmetric in (True, False):
+        error = [float((Q.dequantize_int4(*Q.quantize_int4(w * size, 128, symmetric, torch.float16), 128) / size - w).norm() / w.norm())
+                 for size in (1.0, 1e-4)]
+        # scales of about 4e-5 are steps of 2^-24 apart: at most 2^-24 / 2e-5 = 0.3 % larger
+        assert error[1] <= error[0] * 1.01
+
+
 @pytest.mark.parametrize("zeros", [False, True])
 def test_cpu_path(zeros):
     packed, scales, z = weight(33, 160, 64, zeros, torch.bfloat16)
