@@ -8,18 +8,19 @@
 // rows of the weight as its rows and 8 tokens as its columns. Its order along K is free as long as both sides
 // agree, so a lane takes the pairs (i, i + 4) that a mask leaves in the two halves of a word of eight values, and pairs
 // the activations alike.
-// A nibble masked onto the exponent bits of 1024 is the f16 value 1024 + v, and 1024 + offset comes off each pair,
-// exactly; a high nibble stands for 1024 + 16 v where it is, so a 16th of that less 64 + offset needs no shift. bf16
-// tokens are multiplied as f16 too, by a power of two that brings the largest of a token's values in a warp's K to
-// [2^14, 2^15): a bf16 value has fewer bits than f16's, so all above 2^-28 of the largest are exact, and the others off by
-// at most 2^-39 of it, far below the sum's own f32. (bf16 operands, whose 7 bits need three shifts a word and leave the
-// offset to be taken off the sums, took 65.0 us where this takes 60.2, at 8 x 57344 x 8192, groups of 64; 33.4 and 33.8
-// at 4 x 28672 x 8192; 5.6 and 6.1 at 1 x 4096 x 4096. They turned large tokens into NaN.)
+// A nibble masked into the mantissa of a power of two is that power plus the value (Kim, Henry, Fahim and Hassan Awadalla,
+// "Who Says Elephants Can't Run", 2022, use it for 16-bit operands), and the power and the offset come off each pair,
+// exactly, before the product. f16: 1024 + v; a high nibble stands for 1024 + 16 v where it is, so a 16th of that less
+// 64 + offset needs no shift. bf16: 128 + v, which takes three shifts a word, and of a zero point the lower seven bits, as
+// 128 + 127 is all that 8 bits hold; where a tile has one of 128 and more, that 128 comes off the token's sum by products
+// of its own. So tokens keep their type's range, and a large one on a weight of 0 adds nothing to the sum. (bf16 tokens
+// brought to f16 by a power of two took 33.7 us where this takes 35.7, at 4 x 28672 x 8192 with zero points, 60.4 and 62.8
+// at 8 x 57344 x 8192 in groups of 64, 6.1 and 5.4 at 1 x 4096 x 4096, and lost those below 2^-39 of the largest in 256.)
+// A group's sum is f32 before its scale: of at most 128 values in one warp, so tokens below 2^112 cannot overflow it.
 //
-// Measured: 1 x 4096 x 4096 6.1 us; 4 x 28672 x 8192 with zero points, groups of 128, 33.8 us (3.6 TB/s, 56 % of what a
-// copy reaches); 7 x 128256 x 4096, groups of 64, 62.7 us (4.5 TB/s, 68 %); 16 x 28672 x 8192 49.5 us; 32 tokens 87 us.
-// (Operands of 8 bits were slower at 4 x 28672 x 8192, 57 and 41 us: e4m3, which holds 0 .. 15, is taken apart into
-// 16-bit products on this chip, and whole numbers need three digits of each token and their sums put together.)
+// Measured: 1 x 4096 x 4096 5.4 us; 4 x 28672 x 8192 with zero points, groups of 128, 35.7 us (3.5 TB/s, 53 % of what a
+// copy reaches); 7 x 128256 x 4096 in f16, groups of 64, 62.7 us (4.5 TB/s, 68 %); 16 x 28672 x 8192 50.3 us; 32 tokens
+// 94 us.
 //
 // A warp owns 256 of K for the whole call and keeps its tokens' operand registers; it streams tiles of 32 rows
 // of its K through a ring of TMA copies of its own, with no barrier to other warps. Eight warps make a CTA, a
@@ -63,16 +64,24 @@ struct Int4Args {
 };
 
 // c = A B + (first ? 0 : c): A 16 x 16, B 16 x 8
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
-  if (first)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+#define BRAIN_INT4_MMA(type)                                                                                             \
+  if (first)                                                                                                             \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." type ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};" \
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                        \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));                              \
+  else                                                                                                                   \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." type ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" \
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                        \
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  if constexpr (std::is_same<T, __half>::value) {
+    BRAIN_INT4_MMA("f16.f16")
+  } else {
+    BRAIN_INT4_MMA("bf16.bf16")
+  }
 }
+#undef BRAIN_INT4_MMA
 
 // (w & mask) ^ flip in one operation
 __device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t flip) {
@@ -83,8 +92,11 @@ __device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t fli
 
 // The four pairs (i, i + 4) of a word, less their offset. Two's complement values have their top bit flipped, which
 // makes them an offset of 8. The constants are held in registers.
+template <typename T, bool ZP>
+struct Unpack;
 template <bool ZP>
-struct Unpack {
+struct Unpack<__half, ZP> {
+  static constexpr int kOffset = 255;  // bits of a zero point that an operand takes off itself
   uint32_t mask, flip, high_mask, high_flip;
   __device__ __forceinline__ Unpack() {
     asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
@@ -102,6 +114,25 @@ struct Unpack {
       const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&h), sixteenth, high);
       q[i] = *reinterpret_cast<const uint32_t*>(&a);
       q[i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+};
+template <bool ZP>
+struct Unpack<__nv_bfloat16, ZP> {
+  static constexpr int kOffset = 127;  // 128 + 127 has 8 bits
+  uint32_t mask, flip;
+  __device__ __forceinline__ Unpack() {
+    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(mask));
+    asm volatile("mov.b32 %0, %1;" : "=r"(flip) : "n"(ZP ? 0x43004300 : 0x43084308));
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, int off, uint32_t (&q)[4]) const {
+    const uint32_t less = off * 0x10001 + 0xc300c300;  // twice -128 - off
+    const __nv_bfloat162 one = __float2bfloat162_rn(1.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = pick(w >> (4 * i), mask, flip);
+      const __nv_bfloat162 a = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v), one, *reinterpret_cast<const __nv_bfloat162*>(&less));
+      q[i] = *reinterpret_cast<const uint32_t*>(&a);
     }
   }
 };
@@ -164,15 +195,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   __syncthreads();
   if (split > 1) cluster_arrive_relaxed();
 
-  // ---- this warp's tokens: the pairs of token t * 8 + g, and (bf16) what undoes the factor of tokens t4 * 2, + 1
-  constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
+  // ---- this warp's tokens: the pairs of token t * 8 + g
   uint32_t b[NT][kBlocks][4];
-  float undo[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int m = m0 + t * 8 + g;
     const uint8_t* row = (const uint8_t*)a.x + (m * a.ldx + k0 + t4 * 8) * 2;
-    uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < kBlocks; ++j) {
       uint4 v = make_uint4(0, 0, 0, 0);
@@ -181,29 +209,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
       b[t][j][1] = __byte_perm(v.x, v.z, 0x7632);
       b[t][j][2] = __byte_perm(v.y, v.w, 0x5410);
       b[t][j][3] = __byte_perm(v.y, v.w, 0x7632);
-      // the bits of an absolute value rise with it
-      if (kScaled)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = __vmaxu2(top, b[t][j][i] & 0x7fff7fffu);
-    }
-    if (kScaled) {
-      top = max(top & 0xffffu, top >> 16);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^(14 - e) and its inverse, both normal, for a largest value in [2^e, 2^(e + 1)): e + 127 is top >> 7
-      const int e = max((int)(top >> 7), 15);
-      const float factor = __int_as_float((268 - e) << 23), inverse = __int_as_float((e - 14) << 23);
-#pragma unroll
-      for (int j = 0; j < kBlocks; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float f[2];
-          Words<T>::unpack(b[t][j][i], f);
-          f[0] *= factor, f[1] *= factor;
-          b[t][j][i] = Words<__half>::pack(f);
-        }
-      undo[t][0] = __shfl_sync(0xffffffffu, inverse, t4 * 8);
-      undo[t][1] = __shfl_sync(0xffffffffu, inverse, t4 * 8 + 4);
     }
   }
 
@@ -300,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     }
   };
 
-  const Unpack<ZP> unpack;
+  const Unpack<T, ZP> unpack;
   const uint8_t* wlane = smem + warp * kStages * kTile + g * (kBlocks * 16) + t4 * 4;
   const uint32_t turn = g * 16;  // the copy's swizzle of 16-byte blocks
   int st = 0, parity = 0, meeting = 0, turns = 0;  // meeting: of the round
@@ -325,6 +330,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
             for (int i = 0; i < kZpW; ++i) zpw[h][i] = zpn[h][i];
         }
         if (kAhead && t + 1 < t1) scales(t + 1);
+        // zero points that an operand's offset does not reach: none in 4-bit weights that a quantiser made
+        constexpr bool kFar = ZP && unpack.kOffset < 255;
+        bool far = false;
+        if (kFar) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int h = 0; h < 2 * kHalves; ++h)
+#pragma unroll
+            for (int i = 0; i < kZpW; ++i) top |= zpw[h][i];
+          far = __any_sync(0xffffffffu, (top & 0x80808080u) != 0);
+        }
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
           float acc[kHalves][NT][4];
@@ -336,13 +352,29 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
               uint32_t w[2][4];
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                unpack(*reinterpret_cast<const uint32_t*>(aj + (r * 2 + h) * 8 * (kBlocks * 16)), ZP ? zero_at(r * 2 + h, q) : 8, w[h]);
+                unpack(*reinterpret_cast<const uint32_t*>(aj + (r * 2 + h) * 8 * (kBlocks * 16)), ZP ? zero_at(r * 2 + h, q) & unpack.kOffset : 8, w[h]);
               const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma(acc[r][n], a0, b[n][j][0], b[n][j][1], j == q * kGroupBlocks);
-                mma(acc[r][n], a1, b[n][j][2], b[n][j][3], false);
+                mma<T>(acc[r][n], a0, b[n][j][0], b[n][j][1], j == q * kGroupBlocks);
+                mma<T>(acc[r][n], a1, b[n][j][2], b[n][j][3], false);
               }
+            }
+          }
+          if (kFar && far) {  // the other 128 of them, off each token's sum
+#pragma unroll
+            for (int r = 0; r < kHalves; ++r) {
+              uint32_t w[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) w[h] = zero_at(r * 2 + h, q) > unpack.kOffset ? 0xc300c300 : 0;
+              const uint32_t rest[4] = {w[0], w[1], w[0], w[1]};
+#pragma unroll
+              for (int j = q * kGroupBlocks; j < (q + 1) * kGroupBlocks; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  mma<T>(acc[r][n], rest, b[n][j][0], b[n][j][1], false);
+                  mma<T>(acc[r][n], rest, b[n][j][2], b[n][j][3], false);
+                }
             }
           }
 #pragma unroll
@@ -353,8 +385,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 float& to = sum[h / 2][n][h % 2 * 2 + c];
-                const float v = acc[h / 2][n][h % 2 * 2 + c];
-                to = fmaf(s, kScaled ? v * undo[n][c] : v, to);
+                to = fmaf(s, acc[h / 2][n][h % 2 * 2 + c], to);
               }
           }
         }

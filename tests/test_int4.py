@@ -198,6 +198,48 @@ def test_tokens_of_any_size(zeros):
 
 
 @gpu
+@pytest.mark.parametrize("zeros", [True, False])
+@pytest.mark.parametrize("M,G", [(3, 32), (6, 64), (11, 128)])
+@pytest.mark.parametrize("top,small", [(1.0, 2.0 ** -12), (1.0, 2.0 ** -36), (1.0, 2.0 ** -42), (2.0 ** 60, 2.0 ** -20),
+                                       (2.0 ** 100, 2.0 ** -10)])
+def test_small_tokens_beside_a_large_one_on_a_weight_of_zero(zeros, M, G, top, small):
+    """The large ones add nothing, so the small ones are all of the sum: its bound is theirs."""
+    K = 800
+    packed, scales, z = weight(70, K, G, zeros, torch.bfloat16)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(5)) * small
+    for k in range(5, K, 96):
+        x[:, k] = top * (1 if k % 2 else -1)
+        none = z[:, k // G] if zeros else torch.zeros(70, dtype=torch.uint8)
+        byte = packed[:, k // 2]
+        packed[:, k // 2] = byte & 0x0F | none << 4 if k % 2 else byte & 0xF0 | none
+    x = x.bfloat16()
+    y = Q.int4_linear(x.cuda(), packed.cuda(), scales.cuda(), None if z is None else z.cuda(), group_size=G).cpu()
+    w = dense(packed, scales, z, G)
+    assert (w[:, 5::96] == 0).all()
+    want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    tol = 2.0 ** -8 * want.abs() + (K / 16 + 16) * 2.0 ** -22 * size + 2.0 ** -133  # as above
+    assert ((y.double() - want).abs() <= tol).all(), ((y.double() - want).abs() / tol).max()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,G", [(2, 32), (7, 64), (15, 128)])
+def test_zero_points_of_every_size(dtype, M, G):
+    """All 256 of them, next to one another and in whole tiles of the one or the other side of 128."""
+    packed, scales, _ = weight(512, 1024, G, False, dtype, 6)
+    groups = 1024 // G
+    z = torch.arange(512 * groups).view(groups, 512).t().contiguous() % 256
+    z[:64] = 128
+    z[64:128] = 129
+    z[128:192] = 255
+    z[192:256] = 0
+    z = z.to(torch.uint8)
+    x = torch.randn(M, 1024, generator=torch.Generator().manual_seed(7)).to(dtype)
+    y = Q.int4_linear(x.cuda(), packed.cuda(), scales.cuda(), z.cuda(), group_size=G)
+    check(y, x, dense(packed, scales, z, G), None, dtype)
+
+
+@gpu
 @pytest.mark.parametrize("symmetric", [True, False])
 def test_module(symmetric):
     lin = torch.nn.Linear(512, 96).cuda().bfloat16()
