@@ -161,3 +161,36 @@ def test_feeds_the_fp8_gemms_and_a_graph():
     y = ops.rms_norm(want[2], w, 1e-5).float() @ lin.float().t()
     for out in want[:2]:
         assert (out.float() - y).norm() < 0.06 * y.norm()  # e4m3 on both sides: 2^-4 each at most
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [512, 500, 4096, 5001])
+@pytest.mark.parametrize("scaling", ["rowwise", "block"])
+def test_rows_of_subnormal_size(dtype, D, scaling):
+    """Rows so small that scales stop at 2^-126, and 1 / scale times the row's factor passes f32's range."""
+    if scaling == "block" and D % 128:
+        pytest.skip("blocks of 128")
+    x, _, w = data((4, D), torch.float32, 6, False)
+    x = x / x.abs().amax(-1, keepdim=True) * torch.tensor([1e-39, 2e-40, 1e-38, 1.0])[:, None]
+    x, w = x.to(dtype), w.to(dtype)
+    q, scale = ops.rms_norm_fp8(x.cuda(), w.cuda(), 1e-6, scaling)
+    check(q, scale, None, x, None, w, 1e-6, scaling)
+    assert (scale[:2] == 2.0 ** -126).all() and (q[:3].float() != 0).any(-1).all()
+    # one row offset from 16 bytes against the weight: the kernel for any alignment
+    if scaling == "rowwise":
+        wide = torch.zeros(4, D + 3, dtype=dtype)
+        wide[:, 1:D + 1] = x
+        check(*ops.rms_norm_fp8(wide.cuda()[:, 1:D + 1], w.cuda(), 1e-6), None, x, None, w, 1e-6, scaling)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,ldx,ldr", [(1001, 1001, 1009), (1001, 1009, 1001), (1001, 1002, 1010), (77, 85, 80), (4097, 4105, 4097),
+                                       (1024, 1032, 1024), (1024, 1024, 1025)])
+def test_residual_of_another_row_stride(dtype, D, ldx, ldr):
+    x, r, w = data((7, max(ldx, ldr)), dtype, 5)
+    xs, rs = (t[:, :n].contiguous().cuda()[:, :D] for t, n in ((x, ldx), (r, ldr)))
+    assert xs.stride(0) == ldx and rs.stride(0) == ldr
+    out = ops.add_rms_norm_fp8(xs, rs, w[:D].cuda(), 1e-5)
+    check(*out, x[:, :D], r[:, :D], w[:D], 1e-5, "rowwise")
