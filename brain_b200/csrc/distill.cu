@@ -14,11 +14,10 @@
 // Bound by memory: the logits once for the loss; once in and once out for the gradient. A CTA takes a row and, for
 // the gradient, reads it again right after the first pass, out of L2 (or its own ring); the backward pass of autograd
 // has the log-sum-exp and streams pieces of rows. Measured on bf16 rows of 128256: loss of 2048 89 us (5.9 TB/s),
-// gradient alone 165 us (6.4), loss and gradient of 4096 454 us (4.6). Of the last, the second reading costs 58 us and
-// the writing 80; the two exponentials of a value keep their unit 54 % busy, and a CTA's two passes overlap only with
-// the SM's other CTA's. Holding a row on chip for both passes was slower: 586 us with one CTA of 1024 threads an SM, whose
-// ring keeps three quarters of a row, 560 us with clusters of CTAs that load, exchange their sums and store in turn, and
-// 1300 us as a persistent pipeline of those.
+// gradient alone 165 us (6.4), loss and gradient of 4096 453 us with 100 kept entries a row (4.6), 427 with 20. Of the
+// first, the second reading costs 58 us and the writing 80; the two exponentials of a value keep their unit 54 % busy, and
+// a CTA's two passes overlap only with the SM's other CTA's. A row held on chip for both passes leaves an SM one row at a
+// time, and was slower with one CTA a row and with a cluster.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -523,9 +522,11 @@ int launch(const DistillArgs& a, int64_t M, cudaStream_t st) {
   };
   // Short rows are bound by what a row costs besides its values, so many small CTAs share an SM (64 threads where there are
   // more rows than CTAs of 128 run at once); long ones, and few of them, by what one CTA has in flight. Loss and gradient,
-  // bf16, with 64, 128, 256 and 512 threads: 8192 x 4000 61, 75, 125, 225 us; 4096 x 16000 73, 80, 97, -; 3000 x 24000 90, 84, 91,
-  // 126; 3000 x 32000 119, 112, 108, 134; 2048 x 50257 -, 115, 104, 127; 4096 x 128256 -, 559, 525, 440; 300 x 4000 12.3, 11.7,
-  // 12.3, 16.1; 30 x 100000 43, 27, 22, 22.
+  // 20 kept entries, with 64, 128, 256 and 512 threads, bf16 (f16 within 2 % of it): 8192 x 4000 47, 58, 96, 173 us;
+  // 4096 x 16000 64, 67, 79, 111; 3000 x 24000 80, 73, 76, 104; 3000 x 32000 107, 102, 93, 113; 2048 x 50257 120, 111, 94,
+  // 112; 4096 x 128256 507, 553, 506, 426; 300 x 4000 11.7, 11.1, 11.5, 15.8; 30 x 100000 43, 27, 21, 21. f32: 8192 x 4000
+  // 56, 64, 104, 176; 4096 x 16000 138, 137, 118, 139; 3000 x 32000 209, 219, 178, 171; 2048 x 50257 237, 223, 198, 171;
+  // 2048 x 128256 535, 549, 549, 481.
   const int sms = brain_host::num_sms();
   const auto pick = [&](auto grad) {
     constexpr bool kGrad = decltype(grad)::value;
