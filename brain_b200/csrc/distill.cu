@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
   using W = Words<T>;
   constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
   extern __shared__ __align__(16) float entries[];
-  __shared__ float wm[kRow / 32], ws[kRow / 32], s_kl;
+  __shared__ float wm[kRow / 32], ws[kRow / 32], s_kl, s_near;
   __shared__ int s_any;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % 32;
@@ -310,13 +310,16 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
     asm volatile("bar.arrive 1, %0;" ::"n"(kRow) : "memory");
   } else {
     asm volatile("bar.sync 1, %0;" ::"n"(kRow) : "memory");
-    float top = -INFINITY, sum = 0.f, kl = 0.f;
+    // the student's logits enter the loss less the largest kept one, so what all of a row have in common costs no digits
+    float top = -INFINITY, near = -INFINITY, sum = 0.f, kl = 0.f;
     bool nan = false;
     for (int i = lane; i < a.k; i += 32) {
       top = fmaxf(top, p[i]);
+      if (id[i] >= 0) near = fmaxf(near, zk[i]);
       nan |= p[i] != p[i];
     }
-    top = warp_max(top);
+    top = warp_max(top), near = warp_max(near);
+    if (!(fabsf(near) < INFINITY)) near = 0.f;
     const bool any = __any_sync(0xffffffffu, top > -INFINITY || nan);
     for (int i = lane; i < a.k; i += 32) {
       p[i] = p[i] == -INFINITY ? 0.f : expf(p[i] - top);
@@ -325,12 +328,13 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
     sum = warp_sum(sum);
     for (int i = lane; i < a.k; i += 32) {
       p[i] /= sum;
-      if (id[i] >= 0 && p[i] != 0.f) kl += p[i] * (logf(p[i]) - zk[i] * a.inv_t);
+      if (id[i] >= 0 && p[i] != 0.f) kl += p[i] * (logf(p[i]) - (zk[i] - near) * a.inv_t);
     }
     kl = warp_sum(kl);
     if (lane == 0) {
       s_any = any;
       s_kl = kl;
+      s_near = near;
     }
   }
   int end = -1;
@@ -404,7 +408,8 @@ __global__ void __launch_bounds__(kRow, B) distill_row_kernel(DistillArgs a) {
   const float lse = (m + log2f(s)) * kLn2;
   const bool any = s_any;
   if (tid == 0) {
-    a.loss[row] = any ? a.temp * a.temp * (s_kl + lse) : 0.f;
+    // lse less s_near / T: the fma takes the rounded maximum that the sum is relative to off the exact product
+    a.loss[row] = any ? a.temp * a.temp * (s_kl + (log2f(s) - fmaf(s_near, factor, -m)) * kLn2) : 0.f;
     if (a.lse) a.lse[row] = lse;
     if (a.counts) a.counts[row] = any;
   }

@@ -322,6 +322,19 @@ def test_strides_types_and_shapes(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("T", [1.0, 1.7])
+@pytest.mark.parametrize("offset", [0.0, -3000.0, 2.0 ** 16, -2.0 ** 18])
+def test_loss_of_logits_with_an_offset(offset, T):
+    """What a row's logits have in common changes neither the loss nor how far it is off."""
+    z, t, ids = data(40, 1000, 12, torch.float32, 16)
+    z = z + offset  # rounded to f32, exactly the same for both sides
+    loss = ops.topk_distillation(z.cuda(), t.cuda(), ids.cuda(), T, "none").cpu().double()
+    want = formula(z, t, ids, T)[0]
+    near = z.double() - z.double().amax(-1, keepdim=True)
+    assert ((loss - want).abs() <= tolerances(near.float(), want, want, T, torch.float32)[0]).all(), (loss - want).abs().max()
+
+
+@gpu
 def test_gradient_along_a_direction():
     """The kernel's gradient against differences of the loss in 64 bits."""
     z, t, ids = data(5, 700, 12, torch.float32, 7)
