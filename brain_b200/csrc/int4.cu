@@ -13,9 +13,7 @@
 // exactly, before the product. f16: 1024 + v; a high nibble stands for 1024 + 16 v where it is, so a 16th of that less
 // 64 + offset needs no shift. bf16: 128 + v, which takes three shifts a word, and of a zero point the lower seven bits, as
 // 128 + 127 is all that 8 bits hold; where a tile has one of 128 and more, that 128 comes off the token's sum by products
-// of its own. So tokens keep their type's range, and a large one on a weight of 0 adds nothing to the sum. (bf16 tokens
-// brought to f16 by a power of two took 33.7 us where this takes 35.7, at 4 x 28672 x 8192 with zero points, 60.4 and 62.8
-// at 8 x 57344 x 8192 in groups of 64, 6.1 and 5.4 at 1 x 4096 x 4096, and lost those below 2^-39 of the largest in 256.)
+// of its own. So tokens keep their type's range, and a large one on a weight of 0 adds nothing to the sum.
 // A group's sum is f32 before its scale: of at most 128 values in one warp, so tokens below 2^112 cannot overflow it.
 //
 // Measured: 1 x 4096 x 4096 5.4 us; 4 x 28672 x 8192 with zero points, groups of 128, 35.7 us (3.5 TB/s, 53 % of what a

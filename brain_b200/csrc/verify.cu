@@ -15,9 +15,9 @@
 // positions are touched at one value each. A cluster of CTAs shares a row, as many as fill the GPU at this
 // batch; each warp sums one contiguous segment, with 16-byte loads where the rows start on 16 bytes, and only the
 // segment that holds the border is read again, out of cache. p alone is summed only where p - q is empty.
-// 256 sequences of 128256 f32 ids with draft probabilities take 53 to 56 us (4.7 to 5.0 TB/s), 32 take 11, one of 32000 ids 6.1. The
-// segments' sums are put together warp by warp; a share read from front to back by all warps needs those of all threads,
-// which was slower for few sequences.
+// 256 sequences of 128256 f32 ids with draft probabilities take 53 to 56 us (4.7 to 5.0 TB/s), 32 take 11, one of 32000
+// ids 6.1. The segments' sums are put together warp by warp; a share read from front to back by all warps needs those of
+// all threads, which was slower for few sequences.
 #include <type_traits>
 
 #include "elem.cuh"
